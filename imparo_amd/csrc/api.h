@@ -47,6 +47,20 @@ int imparo_embed_gather(const void* table, int table_dtype, const int32_t* ids, 
 int imparo_place_tokens(int32_t* ids, const int32_t* dst, const int32_t* src, const int32_t* src_index,
                         int n, int vocab, imparo_stream stream);
 
+// The index arrays of a step out of lengths that are on the GPU: row r has lengths[r] tokens in the cache and brings new_tokens[r]
+// (what is negative counts as 0), so its table names need = ceil((length + new) / page_size) pages. The first min(shared[r], need)
+// are those of row leader[r] (or, where that one took them over, of its leader; -1 where there is none such), the others follow one
+// another in `pages`, row after row; -1 behind a row's last page and where `pages` has ended. table [n_rows, width], width as
+// wide as the longest need (what lies beyond is left out). seg_start [n_rows]: where a row's tokens begin; positions, row_of_token and (unless
+// null) slots = page * page_size + place in the page (-1 without a page) [n_tokens]: token by token, up to n_tokens of them; what lies behind
+// the last token is left as it is. lists [n_rows]: the rows that bring one token, then those that bring more. counts [4]: tokens, pages taken
+// from `pages` (more than n_pages: there were too few), rows with one token, rows with more. leader and shared both or neither.
+int imparo_step_tables_max_rows();
+int imparo_step_tables(const int32_t* lengths, const int32_t* new_tokens, const int32_t* leader, const int32_t* shared,
+                       const int32_t* pages, int n_pages, int page_size, int n_rows, int32_t* table, int width,
+                       int32_t* seg_start, int32_t* positions, int32_t* row_of_token, int64_t* slots, int n_tokens,
+                       int32_t* lists, int32_t* counts, imparo_stream stream);
+
 // Row-wise RMS norm. For output row i the source row is rows ? rows[i] : i.
 // If delta is given the row is x + delta[0] + delta[1] + ... first (n_delta
 // slices, each [n_x_rows, width], added in order); with write_back (rows must
@@ -326,6 +340,21 @@ int imparo_attention_decode(const void* q, const void* k_cache, const void* v_ca
                             int heads, int kv_heads, int head_dim, int n_pages, float scale, int window,
                             int n_splits, imparo_stream stream);
 
+// Attention for rows that bring one token each, in groups whose rows have the keys 0 .. shared[g] - 1 in the same pages: those are
+// read once a group, through the table of its first listed row. group_start [n_groups + 1]: group g is the listed rows group_start[g]
+// .. group_start[g + 1] - 1; a listed row in no group shares nothing. Bounds that launches are shaped by, and that must hold: max_shared on
+// shared[g], max_own on the keys a row has behind its group's shared ones, max_group on the rows of a group. The result is the
+// softmax over each row's keys 0 .. position (under `window` the last so many of them; a position below 0 sees nothing and gives
+// zeros); weights are rounded to bfloat16 before they meet the values. part_o [n_rows, heads, parts, head_dim] and part_ml [n_rows,
+// heads, parts, 2] float32 hold the results of parts of the keys, with parts = imparo_attention_shared_parts(...).
+int imparo_attention_shared_parts(int n_rows, int heads, int kv_heads, int n_groups, int max_group, int max_shared, int max_own);
+int imparo_attention_decode_shared(const void* q, const void* k_cache, const void* v_cache, void* out, float* part_o,
+                                   float* part_ml, const int32_t* rows, int n_rows, const int32_t* group_start, int n_groups,
+                                   const int32_t* shared, const int32_t* seg_start, const int32_t* positions,
+                                   const int32_t* block_table, int table_stride, int page_size, int heads, int kv_heads,
+                                   int head_dim, int n_pages, float scale, int window, int max_shared, int max_own,
+                                   int max_group, imparo_stream stream);
+
 // The same for a step whose rows' keys and values are not in the cache yet: qkv is the fused
 // projection's float32 rows [tokens, (heads + 2 kv_heads) x head_dim] (q heads, k heads, v heads). The
 // launch norms each head of q and k (weights [head_dim], or both null: no norm), rotates them
@@ -459,6 +488,13 @@ int imparo_argmax_rows(const float* logits, int32_t* out, int n_rows, int vocab,
 // reaches uniform[r]; temperature <= 0 is argmax.
 int imparo_sample_rows(const float* logits, const float* temperature, const float* uniform, int32_t* out,
                        int n_rows, int vocab, imparo_stream stream);
+// The same under filters, each one value a row or null: top_k (0 or less, vocab or more: off) keeps the top_k largest logits, top_p
+// (1 and above: off) of those the fewest largest ones whose probabilities reach top_p of theirs together, min_p (0: off) of
+// those the ones with at least min_p times the largest probability; equal logits count in the order of their indices. Weights are
+// held as integers of 2^-44 of the largest, and what is below that is not drawn. A row without a filter gets the pick of
+// imparo_sample_rows. At most 2^19 logits a row, in any 4-byte alignment.
+int imparo_pick_rows(const float* logits, const float* temperature, const float* uniform, const int32_t* top_k, const float* top_p,
+                     const float* min_p, int32_t* out, int n_rows, int vocab, imparo_stream stream);
 
 // Fills n float32 values (or n int32 values of the same bits) without a memset node.
 int imparo_fill_f32(float* p, float value, int64_t n, imparo_stream stream);

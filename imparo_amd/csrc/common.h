@@ -224,6 +224,7 @@ __device__ __forceinline__ void wave_lds_sync() {
 // One per file of kernels: loads that file's code onto the current device (imparo_load_code calls them all).
 int imparo_load_code_attention();
 int imparo_load_code_attention_mfma();
+int imparo_load_code_attention_shared();
 int imparo_load_code_decay_scan();
 int imparo_load_code_decode_rows();
 int imparo_load_code_diff_attention();
@@ -238,6 +239,7 @@ int imparo_load_code_row_ops();
 int imparo_load_code_sampling();
 int imparo_load_code_selective_scan();
 int imparo_load_code_some_rows();
+int imparo_load_code_step_tables();
 int imparo_load_code_streams();
 
 static inline int launch_status() {

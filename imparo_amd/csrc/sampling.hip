@@ -131,18 +131,15 @@ extern "C" int imparo_argmax_rows(const float* logits, int32_t* out, int n_rows,
 // values a time, and all that is no addition (exponentials, comparisons) is done by the whole block. Measured, 64
 // rows of 65,536 logits: 153 us with both chains reading LDS and memory value by value, 38 us so (28 us for rows of 16,384).
 #define SAMPLE_THREADS 1024
-__global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_rows(
-    const float* __restrict__ logits, const float* __restrict__ temperature, const float* __restrict__ uniform,
-    int32_t* __restrict__ out, int vocab) {
+__device__ __forceinline__ void sample_row(const float* __restrict__ row, float temp, float uniform, int32_t* __restrict__ out,
+                                           int vocab) {
     __shared__ Best scratch[16];
     __shared__ __attribute__((aligned(16))) float sums[SAMPLE_THREADS], before[SAMPLE_THREADS];
     __shared__ int first_past, last_positive, found;
     __shared__ float cum_shared, target_shared;
-    const float* row = logits + (size_t)blockIdx.x * vocab;
     const Best top = row_best(row, vocab, scratch);
-    const float temp = temperature[blockIdx.x];
     if (!(temp > 0.f)) {
-        if (threadIdx.x == 0) out[blockIdx.x] = top.i;
+        if (threadIdx.x == 0) *out = top.i;
         return;
     }
     const float inv_t = 1.0f / temp;
@@ -200,7 +197,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_rows(
                 *reinterpret_cast<float4*>(&before[t + 4 * j]) = b;
             }
         }
-        target_shared = uniform[blockIdx.x] * total;
+        target_shared = uniform * total;
     }
     __syncthreads();
     const float target = target_shared;
@@ -243,7 +240,13 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_rows(
         __syncthreads();
         if (found >= 0) break;
     }
-    if (tid == 0) out[blockIdx.x] = found >= 0 ? found : last;
+    if (tid == 0) *out = found >= 0 ? found : last;
+}
+
+__global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_rows(
+    const float* __restrict__ logits, const float* __restrict__ temperature, const float* __restrict__ uniform,
+    int32_t* __restrict__ out, int vocab) {
+    sample_row(logits + (size_t)blockIdx.x * vocab, temperature[blockIdx.x], uniform[blockIdx.x], out + blockIdx.x, vocab);
 }
 
 extern "C" int imparo_sample_rows(const float* logits, const float* temperature, const float* uniform, int32_t* out,
@@ -252,6 +255,400 @@ extern "C" int imparo_sample_rows(const float* logits, const float* temperature,
     if (n_rows == 0) return IMPARO_OK;
     const int threads = vocab >= 16384 ? SAMPLE_THREADS : 256;
     k_sample_rows<<<n_rows, threads, 0, (hipStream_t)stream>>>(logits, temperature, uniform, out, vocab);
+    return launch_status();
+}
+
+// ---------------------------------------------------------------- picks under top-k, top-p and min-p
+// With m the row's largest logit, w_i = 2^((x_i - m) log2(e) / T) and tokens in the order "larger logit first, smaller index
+// first": top-k keeps the first k, top-p of those the fewest first whose weights reach p of their sum, min-p of those the ones
+// with w_i >= min_p. Each keeps a beginning of that order, so what is kept is all above a logit and so many ties with it, the
+// ones of the smallest index. The pick is the first token, in the order of indices, whose running sum of kept weights passes u
+// times their sum.
+// Sums decide here, and which token a sum passes at must not depend on how it was split: a weight is held as the integer
+// nearest to w 2^44 (w from a float64 exponential), so sums are exact in any order, over any split, and by atomics. 2^19 logits
+// fill 63 bits. A token below 2^-44 of the likeliest is not drawn: all of those together weigh less than 2^-25, under one
+// step of a 24-bit u.
+// The border is found without sorting: a histogram in LDS, linear in the logit over the range that weighs anything, a scan for the bin
+// where the count (or the weight) is reached, and the same again inside that bin over its keys' bits until one key is left.
+// One block a row, which reads it again for each pass (out of L2).
+#define PICK_BINS 2048
+#define PICK_LIST 2048
+#define PICK_CUT 44
+
+typedef unsigned long long u64;
+
+// the float's place in the order of floats
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+
+// 2^y 2^44 to the nearest integer, y <= 0 (0 below 2^-44.5): 2^f = e^(f ln 2) of the fraction |f| <= 1/2 as its power series, cut where the next
+// term is below 2^-47, then scaled by the exponent and rounded by an addition of 2^52
+__device__ __forceinline__ u64 weight_of(double y) {
+    const double k = rint(y), f = (y - k) * 0.69314718055994530942;
+    double p = fma(f, 1.0 / 39916800.0, 1.0 / 3628800.0);
+    p = fma(f, p, 1.0 / 362880.0);
+    p = fma(f, p, 1.0 / 40320.0);
+    p = fma(f, p, 1.0 / 5040.0);
+    p = fma(f, p, 1.0 / 720.0);
+    p = fma(f, p, 1.0 / 120.0);
+    p = fma(f, p, 1.0 / 24.0);
+    p = fma(f, p, 1.0 / 6.0);
+    p = fma(f, p, 0.5);
+    p = fma(f, p, 1.0);
+    p = fma(f, p, 1.0);
+    const double scaled = __hiloint2double(__double2hiint(p) + (((int)k + PICK_CUT) << 20), __double2loint(p));
+    return y < -(PICK_CUT + 0.5) ? 0 : (u64)__double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+}
+
+template <int N>
+__device__ __forceinline__ u64 lane_xor_u64(u64 v) {
+    return ((u64)lane_xor_bits<N>((uint32_t)(v >> 32)) << 32) | lane_xor_bits<N>((uint32_t)v);
+}
+__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
+    v += lane_xor_u64<1>(v);
+    v += lane_xor_u64<2>(v);
+    v += lane_xor_u64<4>(v);
+    v += lane_xor_u64<8>(v);
+    v += lane_xor_u64<16>(v);
+    v += lane_xor_u64<32>(v);
+    return v;
+}
+__device__ __forceinline__ u64 wave_scan_u64(u64 v) {             // the sum over the lanes up to and with this one
+    const int lane = threadIdx.x & (WAVE - 1);
+#pragma unroll
+    for (int n = 1; n < WAVE; n <<= 1) {
+        const u64 below = __shfl_up(v, n, WAVE);
+        if (lane >= n) v += below;
+    }
+    return v;
+}
+
+struct PickShared {
+    u64 hist[PICK_BINS];
+    uint32_t list[PICK_LIST];
+    u64 waves[16];
+    float tops[16], lows[16];
+    u64 above, inside, total, need;   // of the bin where the sum is reached: what lies above it, what it holds; all there is; what is asked for
+    int bin, n_list;
+    uint32_t key_low, key_high;
+    int cut;
+};
+
+// The bin of sh.hist where the running sum reaches what is asked for: `need`, or for share >= 0 that share of all. Leaves bin,
+// above, inside, total and need in LDS; every thread calls, behind and ahead of a barrier of its own.
+__device__ __forceinline__ void pick_bin(PickShared& sh, u64 need, double share) {
+    const int threads = blockDim.x, per = PICK_BINS / threads, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    u64 mine = 0;
+    for (int i = 0; i < per; ++i) mine += sh.hist[tid * per + i];
+    const u64 upto = wave_scan_u64(mine);
+    if (lane == WAVE - 1) sh.waves[wave] = upto;
+    __syncthreads();
+    u64 before = 0, total = 0;
+    for (int w = 0; w < threads / WAVE; ++w) {
+        const u64 v = sh.waves[w];
+        before += w < wave ? v : 0;
+        total += v;
+    }
+    if (share >= 0.0) need = max((u64)1, (u64)ceil(share * (double)total));
+    u64 at = before + upto - mine;
+    if (at < need && need <= at + mine) {
+        int b = tid * per;
+        u64 v = sh.hist[b];
+        while (at + v < need) {
+            at += v;
+            v = sh.hist[++b];
+        }
+        sh.bin = b;
+        sh.above = at;
+        sh.inside = v;
+        sh.total = total;
+        sh.need = need;
+    }
+    __syncthreads();
+}
+
+// A row's logits, lane by lane: wave w has the values of its own run, 256 a turn, four neighbours a lane. What stands in front of
+// the row or behind it inside the 16 aligned bytes that hold its first or last value is read with them (the same 16 bytes of
+// memory, so it is there) and counts as -inf, as NaN does.
+#define PICK_DEEP 8
+struct PickRow {
+    const float4* base;
+    int skew, vocab, turns, first;      // first: index in the row of this lane's first value in turn 0
+
+    __device__ __forceinline__ void open(const float* row, int n) {
+        vocab = n;
+        skew = (int)(((uintptr_t)row & 15) >> 2);
+        base = reinterpret_cast<const float4*>(row - skew);
+        const int waves = blockDim.x / WAVE, lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+        turns = (vocab + skew + 4 * WAVE * waves - 1) / (4 * WAVE * waves);
+        first = wave * turns * 4 * WAVE + 4 * lane - skew;
+    }
+    // f(values, index of the first of the four), turn after turn, the loads of PICK_DEEP turns in flight
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        for (int c0 = 0; c0 < turns; c0 += PICK_DEEP) {
+            float4 v[PICK_DEEP];
+#pragma unroll
+            for (int c = 0; c < PICK_DEEP; ++c)
+                v[c] = base[min(max(first + skew + (c0 + c) * 4 * WAVE, 0), vocab + skew - 1) >> 2];
+#pragma unroll
+            for (int c = 0; c < PICK_DEEP; ++c) {
+                if (c0 + c >= turns) break;
+                const int i = first + (c0 + c) * 4 * WAVE;
+                float x[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool on = i + j >= 0 && i + j < vocab && x[j] == x[j];
+                    x[j] = on ? x[j] + 0.f : -INFINITY;          // (+ 0: -0 and 0 are one value)
+                }
+                f(x, i);
+            }
+        }
+    }
+};
+
+// What of a row is kept: keys above `key`, and the key itself up to index `cut`
+struct PickSet {
+    uint32_t key;
+    int cut;
+    __device__ __forceinline__ bool has(uint32_t k, int index) const { return k > key || (k == key && index <= cut); }
+};
+
+// Narrows `set` to the beginning of its order where the count (COUNT) reaches `need`, or the weights the share `share` of theirs.
+template <bool COUNT>
+__device__ __forceinline__ void pick_narrow(PickShared& sh, const PickRow& row, PickSet& set, float top, float bin_scale,
+                                            float reach, float c1f, double c1, u64 need, double share) {
+    const int tid = threadIdx.x, threads = blockDim.x;
+    auto weight = [&](float x) { return COUNT ? (u64)1 : weight_of(((double)x - (double)top) * c1); };
+    auto bin_of = [&](float x) { return (int)fminf((top - x) * bin_scale, (float)(PICK_BINS - 1)); };
+    for (int b = tid; b < PICK_BINS; b += threads) sh.hist[b] = 0;
+    if (tid == 0) {
+        sh.n_list = 0;
+        sh.key_low = 0xFFFFFFFFu;
+        sh.key_high = 0;
+        sh.total = 0;
+    }
+    __syncthreads();
+    row.each([&](const float (&x)[4], int index) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (x[j] >= reach && set.has(key_of(x[j]), index + j)) atomicAdd(&sh.hist[bin_of(x[j])], weight(x[j]));
+    });
+    __syncthreads();
+    pick_bin(sh, need, share);
+    if (sh.total == 0) return;                                    // fewer than are asked for: all stay
+    u64 above = sh.above;
+    need = sh.need;
+    const int bin = sh.bin;
+    row.each([&](const float (&x)[4], int index) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (!(x[j] >= reach) || bin_of(x[j]) != bin) continue;
+            const uint32_t k = key_of(x[j]);
+            if (!set.has(k, index + j)) continue;
+            const int at = atomicAdd(&sh.n_list, 1);
+            if (at < PICK_LIST) sh.list[at] = k;
+            atomicMin(&sh.key_low, k);
+            atomicMax(&sh.key_high, k);
+        }
+    });
+    __syncthreads();
+    const int n_list = sh.n_list;
+    uint32_t low = sh.key_low, high = sh.key_high;
+    u64 inside = sh.inside;
+    while (low != high) {                                         // (at most three times: 11 bits of at most 32 each)
+        const int bits = 32 - __clz((int)(high - low)), shift = max(0, bits - 11);
+        __syncthreads();
+        for (int b = tid; b < PICK_BINS; b += threads) sh.hist[b] = 0;
+        __syncthreads();
+        auto float_of = [](uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); };
+        if (n_list <= PICK_LIST) {
+            for (int i = tid; i < n_list; i += threads) {
+                const uint32_t k = sh.list[i];
+                if (k >= low && k <= high) atomicAdd(&sh.hist[(high - k) >> shift], weight(float_of(k)));
+            }
+        } else {
+            row.each([&](const float (&x)[4], int index) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t k = key_of(x[j]);
+                    if (x[j] >= reach && k >= low && k <= high && set.has(k, index + j)) atomicAdd(&sh.hist[(high - k) >> shift], weight(x[j]));
+                }
+            });
+        }
+        __syncthreads();
+        pick_bin(sh, need - above, -1.0);
+        above += sh.above;
+        inside = sh.inside;
+        high -= (uint32_t)sh.bin << shift;
+        low = high - low > (1u << shift) - 1 ? high - ((1u << shift) - 1) : low;
+    }
+    // one key is left: so many of its tokens, in the order of their indices, reach what is asked for
+    const u64 each = weight(__uint_as_float(high & 0x80000000u ? high ^ 0x80000000u : ~high));
+    const u64 ties = (need - above + each - 1) / each;
+    const PickSet old = set;
+    set.key = high;
+    set.cut = INT_MAX;
+    if (ties * each >= inside) {                                  // all of them
+        if (high == old.key) set.cut = old.cut;
+        return;
+    }
+    const int lane = tid & (WAVE - 1), wave = tid / WAVE;
+    u64 mine = 0;
+    row.each([&](const float (&x)[4], int index) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine += __popcll(__ballot(x[j] >= reach && key_of(x[j]) == high));
+    });
+    if (lane == 0) sh.waves[wave] = mine;
+    __syncthreads();
+    u64 before = 0;
+    for (int w = 0; w < wave; ++w) before += sh.waves[w];
+    if (before < ties && ties <= before + mine) {
+        row.each([&](const float (&x)[4], int index) {
+            u64 ahead = before;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool on = x[j] >= reach && key_of(x[j]) == high;
+                const u64 who = __ballot(on);
+                ahead += __popcll(who & ((1ull << lane) - 1));
+                before += __popcll(who);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (x[j] >= reach && key_of(x[j]) == high && ++ahead == ties) sh.cut = index + j;
+        });
+    }
+    __syncthreads();
+    set.cut = sh.cut;
+}
+
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void k_pick_rows(
+    const float* __restrict__ logits, const float* __restrict__ temperature, const float* __restrict__ uniform,
+    const int32_t* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p,
+    int32_t* __restrict__ out, int vocab) {
+    __shared__ PickShared sh;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    const float* row_at = logits + (size_t)r * vocab;
+    const float temp = temperature[r], u = uniform[r];
+    const int k = top_k ? top_k[r] : 0;
+    const float p = top_p ? top_p[r] : 1.f, mp = min_p ? min_p[r] : 0.f;
+    const bool by_k = k > 0 && k < vocab, by_p = p < 1.f, by_m = mp > 0.f;
+    if (!(temp > 0.f) || !(by_k || by_p || by_m)) {               // greedy, or the whole distribution
+        sample_row(row_at, temp, u, out + r, vocab);
+        return;
+    }
+    PickRow row;
+    row.open(row_at, vocab);
+    float top = -INFINITY, low = INFINITY;
+    row.each([&](const float (&x)[4], int) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            top = fmaxf(top, x[j]);
+            low = fminf(low, x[j] > -INFINITY ? x[j] : INFINITY);
+        }
+    });
+    top = wave_max(top);
+    low = -wave_max(-low);
+    if (lane == 0) {
+        sh.tops[wave] = top;
+        sh.lows[wave] = low;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / WAVE; ++w) {
+        top = fmaxf(top, sh.tops[w]);
+        low = fminf(low, sh.lows[w]);
+    }
+    if (!(top < INFINITY) || !(top > -INFINITY)) {                // an infinite logit takes it, or there is none to take
+        sample_row(row_at, 0.f, u, out + r, vocab);
+        return;
+    }
+    const double c1 = 1.44269504088896340736 / (double)temp;
+    const float c1f = fminf((float)c1, 3.0e38f);
+    // logits below `reach` weigh nothing; a token that min-p takes out is not looked at again either, as every smaller one goes too
+    const double floor_y = by_m ? fmax(-(double)PICK_CUT, log2((double)fminf(mp, 1.f))) : -(double)PICK_CUT;
+    const float span = fminf(top - low, (float)PICK_CUT / c1f);
+    const float reach = fmaxf(low, top - (float)PICK_CUT / c1f);
+    const float bin_scale = span > 1e-30f && span < 1e30f ? (float)PICK_BINS * 0.99999f / span : 0.f;
+    PickSet set{0u, INT_MAX};
+    if (by_k) pick_narrow<true>(sh, row, set, top, bin_scale, reach, c1f, c1, (u64)k, -1.0);
+    __syncthreads();
+    if (by_p) pick_narrow<false>(sh, row, set, top, bin_scale, reach, c1f, c1, 0, (double)fmaxf(p, 0.f));
+    __syncthreads();
+
+    // ---- the pick: sums over the waves' runs, then inside the run where u falls
+    auto kept = [&](float x, int index) {
+        return x >= reach && set.has(key_of(x), index) && ((double)x - (double)top) * c1 >= floor_y;
+    };
+    u64 mine = 0;
+    int last = -1;
+    row.each([&](const float (&x)[4], int index) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (kept(x[j], index + j)) {
+                mine += weight_of(((double)x[j] - (double)top) * c1);
+                last = index + j;
+            }
+    });
+    mine = wave_sum_u64(mine);
+    if (lane == 0) sh.waves[wave] = mine;
+    if (tid == 0) sh.cut = -1;
+    __syncthreads();
+    u64 before = 0, total = 0;
+    for (int w = 0; w < THREADS / WAVE; ++w) {
+        before += w < wave ? sh.waves[w] : 0;
+        total += sh.waves[w];
+    }
+    const double want = fmax((double)u * (double)total, 0.0);     // (a NaN is 0)
+    if (!(want < (double)total)) {                                // u of 1: the last token that is kept
+        if (last >= 0) atomicMax(&sh.cut, last);
+        __syncthreads();
+        if (tid == 0) out[r] = sh.cut;
+        return;
+    }
+    const u64 target = min((u64)want, total - 1);
+    if (before <= target && target < before + mine) {
+        int found = -1;
+        row.each([&](const float (&x)[4], int index) {
+            if (found >= 0) return;
+            u64 w[4], four = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = kept(x[j], index + j) ? weight_of(((double)x[j] - (double)top) * c1) : 0;
+                four += w[j];
+            }
+            if (!__any(four != 0)) return;
+            const u64 upto = wave_scan_u64(four);
+            const u64 past = __ballot(before + upto > target);
+            if (past) {
+                u64 at = before + upto - four;
+                int pick = -1;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    at += w[j];
+                    if (pick < 0 && at > target) pick = index + j;
+                }
+                found = __shfl(pick, __ffsll((long long)past) - 1, WAVE);
+            }
+            before += __shfl(upto, WAVE - 1, WAVE);
+        });
+        if (lane == 0) out[r] = found;
+    }
+}
+
+extern "C" int imparo_pick_rows(const float* logits, const float* temperature, const float* uniform, const int32_t* top_k,
+                                const float* top_p, const float* min_p, int32_t* out, int n_rows, int vocab,
+                                imparo_stream stream) {
+    if (n_rows < 0 || vocab <= 0 || vocab > 1 << 19) return IMPARO_BAD_ARGUMENT;
+    if (n_rows == 0) return IMPARO_OK;
+    if (!logits || !temperature || !uniform || !out || ((uintptr_t)logits & 3)) return IMPARO_BAD_ARGUMENT;
+    hipStream_t s = (hipStream_t)stream;
+    // (a row without a filter goes through sample_row, whose sums depend on the threads: as many as imparo_sample_rows has)
+    if (vocab >= 16384) k_pick_rows<1024><<<n_rows, 1024, 0, s>>>(logits, temperature, uniform, top_k, top_p, min_p, out, vocab);
+    else k_pick_rows<256><<<n_rows, 256, 0, s>>>(logits, temperature, uniform, top_k, top_p, min_p, out, vocab);
     return launch_status();
 }
 

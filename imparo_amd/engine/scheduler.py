@@ -20,7 +20,7 @@ import os
 from dataclasses import dataclass, field
 from typing import Callable, Dict, Hashable, List, Optional, Sequence, Tuple
 
-from ..sampling.sampler import SamplingParams, uniform_for
+from ..sampling.sampler import NO_FILTERS, SamplingParams, uniform_for
 
 DEFAULT_PORTION = 512   # the reference's prefill chunk (crates/imparo-model/src/lib.rs:1000)
 
@@ -67,7 +67,8 @@ class Planned:
 class Scheduler:
     """`engine` needs: step(entries) -> logits rows or None, release(id),
     cache (a CacheManager), page_size. `pick(logits, temperatures, uniforms)`
-    turns logits rows into token ids.
+    turns logits rows into token ids; where a request of the step asks for top-k,
+    top-p or min-p it is given every row's (top_k, top_p, min_p) as a fourth argument.
 
     The decisions (whom to admit, what each request feeds under the budget,
     whom to pre-empt) are taken by the native scheduler core
@@ -246,13 +247,15 @@ class Scheduler:
             return self._read_back()
         temps = [r.params.temperature for r in askers]
         unis = [uniform_for(r.params.seed, r.drawn) for r in askers]
+        filters = [r.params.filters for r in askers]
+        asked = (logits, temps, unis) if all(f == NO_FILTERS for f in filters) else (logits, temps, unis, filters)
         if self.pick_async is not None:
-            pending = self.pick_async(logits, temps, unis)
+            pending = self.pick_async(*asked)
             out = self._read_back()          # the step before's tokens, while this step runs
             self._count_unread(askers, pending)
             return out
         out: List[Tuple[Hashable, int]] = []
-        picks = self.pick(logits, temps, unis)
+        picks = self.pick(*asked)
         for r, tok in zip(askers, picks):
             tok = int(tok)
             h = self.engine.cache.handle(r.id)
@@ -346,7 +349,8 @@ def generate(model, input_ids: Sequence[Sequence[int]], max_tokens: int = 16, te
              seed: int = 0, stop_token_ids: Optional[Sequence[int]] = None, dtype: str = "bfloat16",
              ctx: Optional[int] = None, parallel: int = 64, max_batch_tokens: int = 2048,
              page_size: int = 64, overlap: bool = True, num_pages=None,
-             kv_budget_bytes: Optional[int] = None) -> List[List[int]]:
+             kv_budget_bytes: Optional[int] = None, top_k: int = 0, top_p: float = 1.0,
+             min_p: float = 0.0) -> List[List[int]]:
     """Tokens in, tokens out. `model` is a model folder or an Engine; returns
     the generated ids of every prompt, in order. Request `i` samples with seed
     `seed + i`. `ctx` is the most tokens one request may hold (the reference's
@@ -354,9 +358,11 @@ def generate(model, input_ids: Sequence[Sequence[int]], max_tokens: int = 16, te
     `overlap`: queue each step before the tokens of the step before are read
     back (the same tokens come out; False waits after every step).
     `num_pages` or `kv_budget_bytes` size the cache pools instead of `ctx` and
-    `parallel` (a smaller pool makes requests wait or be recomputed)."""
+    `parallel` (a smaller pool makes requests wait or be recomputed).
+    `top_k`, `top_p`, `min_p`: as in SamplingParams, for every request."""
     from .engine import Engine
     from ..sampling.sampler import Sampler
+    SamplingParams(top_k=top_k, top_p=top_p, min_p=min_p)       # (refused before a model is loaded)
     if len(input_ids) == 0:
         return []
     if isinstance(model, Engine):
@@ -377,7 +383,7 @@ def generate(model, input_ids: Sequence[Sequence[int]], max_tokens: int = 16, te
                       pick_async=sampler.pick_async if overlap else None)
     for i, prompt in enumerate(input_ids):
         sched.add(i, prompt, SamplingParams(temperature=temperature, max_tokens=max_tokens, seed=seed + i,
-                                            stop_token_ids=stops))
+                                            stop_token_ids=stops, top_k=top_k, top_p=top_p, min_p=min_p))
         if sched.finished.get(i) is not None and sched.finished[i].finish_reason.startswith("error"):
             raise ValueError(f"request {i}: {sched.finished[i].finish_reason[7:]}")
     done = sched.run()

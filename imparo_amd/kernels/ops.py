@@ -49,6 +49,12 @@ def _dev(t: Optional[torch.Tensor], what: str, dtype=None, shape=None) -> int:
     return t.data_ptr()
 
 
+def _here(t: torch.Tensor, what: str) -> None:
+    """Refuses a tensor of another GPU than the current one, whose stream the launch goes to."""
+    if t.device.type == "cuda" and t.device.index != torch.cuda.current_device():
+        raise KernelArgumentError(f"{what} is on {t.device}, the current device is {torch.cuda.current_device()}")
+
+
 _launch_stream: Optional[int] = None
 
 
@@ -231,6 +237,43 @@ def place_tokens(ids: torch.Tensor, dst: torch.Tensor, src: torch.Tensor, src_in
         _dev(src, "sampled tokens", torch.int32), _dev(src_index, "indices of sampled tokens", torch.int32, (n,)),
         n, vocab, _stream()), "place_tokens")
     return ids
+
+
+def step_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, pages: torch.Tensor, page_size: int, block_table: torch.Tensor,
+                seg_start: torch.Tensor, positions: torch.Tensor, row_of_token: torch.Tensor, slots: Optional[torch.Tensor],
+                lists: torch.Tensor, counts: torch.Tensor, leader: Optional[torch.Tensor] = None,
+                shared: Optional[torch.Tensor] = None):
+    """The index arrays of a step out of lengths on the GPU. Row r has lengths[r] tokens in the cache and brings new_tokens[r]; its
+    table names the pages of them all: with `leader` and `shared` the first shared[r] pages are those of row leader[r] (which took them
+    over itself or has them of its own), the others come out of `pages`, row after row. Fills and returns block_table [rows, width] (-1
+    behind a row's last page and where `pages` has ended; width: as wide as the longest row needs), seg_start [rows], positions,
+    row_of_token [tokens] and slots (int64 [tokens] or None: page * page_size + place inside it), lists [rows] (the rows that bring one
+    token, then those that bring more) and counts [4]: tokens, pages taken from `pages`, rows with one token, rows with more. Where
+    there are fewer tokens (or rows in the list) than room, the rest is left as it was; where there is too little room the arrays
+    hold what fits and counts says what was needed."""
+    n = lengths.shape[0]
+    if page_size < 1 or page_size & (page_size - 1) or page_size > 1 << 30:
+        raise KernelArgumentError(f"step_tables: page size must be a power of two, got {page_size}")
+    if (leader is None) != (shared is None):
+        raise KernelArgumentError("step_tables: leaders and shared pages are given together")
+    if n > library().imparo_step_tables_max_rows():
+        raise KernelArgumentError(f"step_tables: {n} rows; at most {library().imparo_step_tables_max_rows()} are taken")
+    if block_table.dim() != 2 or block_table.shape[1] < 1 or positions.dim() != 1 or pages.dim() != 1:
+        raise KernelArgumentError("step_tables: a [rows, pages] block table and one position a token are needed")
+    _here(lengths, "lengths")
+    n_tokens = positions.shape[0]
+    args = (_dev(lengths, "lengths", torch.int32, (n,)), _dev(new_tokens, "new tokens", torch.int32, (n,)),
+            _dev(leader, "leaders", torch.int32, (n,)), _dev(shared, "shared pages", torch.int32, (n,)),
+            _dev(pages, "pages", torch.int32), pages.shape[0], page_size, n,
+            _dev(block_table, "block table", torch.int32, (n, block_table.shape[1])), block_table.shape[1],
+            _dev(seg_start, "seg_start", torch.int32, (n,)), _dev(positions, "positions", torch.int32),
+            _dev(row_of_token, "row_of_token", torch.int32, (n_tokens,)), _dev(slots, "slots", torch.int64, (n_tokens,)), n_tokens,
+            _dev(lists, "lists", torch.int32, (n,)), _dev(counts, "counts", torch.int32, (4,)))
+    if n == 0:
+        counts.zero_()
+    else:
+        _check(library().imparo_step_tables(*args, _stream()), "step_tables")
+    return block_table, seg_start, positions, row_of_token, slots, lists, counts
 
 
 def dynamic_tanh(x: torch.Tensor, alpha: float, weight: torch.Tensor, bias: torch.Tensor, out: torch.Tensor,
@@ -547,6 +590,53 @@ def attention_decode(q, k_cache, v_cache, out, part_o, part_ml, rows, n_rows: in
     return out
 
 
+def attention_shared_parts(n_rows: int, heads: int, kv_heads: int, head_dim: int, n_groups: int, max_group: int, max_shared: int,
+                           max_own: int) -> int:
+    """Into how many parts `attention_decode_shared` cuts the keys of a row under these bounds: its scratch holds one entry a part."""
+    if head_dim % 16 or not 0 < head_dim <= 128 or kv_heads <= 0 or heads <= 0 or heads % kv_heads:
+        raise KernelArgumentError(f"attention_shared_parts: {heads} heads of {head_dim} by {kv_heads} are not taken")
+    if min(n_rows, n_groups, max_group, max_shared, max_own) < 0 or max(max_shared, max_own) > 1 << 30:
+        raise KernelArgumentError("attention_shared_parts: a bound is negative, or above 2^30")
+    return int(library().imparo_attention_shared_parts(int(n_rows), int(heads), int(kv_heads), int(n_groups), int(max_group),
+                                                       int(max_shared), int(max_own)))
+
+
+def attention_decode_shared(q, k_cache, v_cache, out, part_o, part_ml, rows, n_rows: int, group_start, shared, seg_start, positions,
+                            block_table, scale: float, window: Optional[int], max_shared: int, max_own: int,
+                            max_group: int) -> torch.Tensor:
+    """`attention_decode` for rows in groups that share a prefix: group g is the listed rows group_start[g] .. group_start[g + 1] - 1,
+    whose tables name the same pages for the keys 0 .. shared[g] - 1 (any number of them; where it ends inside a page, that page's
+    part). Those keys are read once a group, through its first row's table, the ones behind by each row; a listed row in no group
+    shares nothing. The bounds shape the launch, so that it can be captured while groups, shares and positions change on the device, and
+    must hold: shared[g] <= max_shared, position + 1 - shared[g] <= max_own, rows of a group <= max_group. `part_o` [n_rows, heads, parts,
+    head_dim] and `part_ml` [n_rows, heads, parts, 2] float32 are scratch, parts = attention_shared_parts(...); launches that may run
+    at once need scratch of their own. A row whose position is below 0 sees nothing and is zeros; rows that are not listed are left as
+    they are."""
+    n, heads, head_dim, n_pages, kv_heads, page_size = _check_mfma(q, k_cache, v_cache, out)
+    _here(q, "q")
+    if window is not None and window < 1:
+        raise KernelArgumentError(f"attention_decode_shared: a window of {window} keys; at least 1, or None for all")
+    if rows.dim() != 1 or not 0 <= n_rows <= rows.shape[0]:
+        raise KernelArgumentError(f"attention_decode_shared: {n_rows} rows are listed in {list(rows.shape)}")
+    if group_start.dim() != 1 or group_start.shape[0] < 1:
+        raise KernelArgumentError("attention_decode_shared: group_start has one entry more than there are groups")
+    n_groups = group_start.shape[0] - 1
+    if seg_start.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] != seg_start.shape[0] or block_table.shape[1] < 1:
+        raise KernelArgumentError(f"attention_decode_shared: a block table of {list(block_table.shape)} does not go with "
+                                  f"{list(seg_start.shape)} rows")
+    parts = attention_shared_parts(n_rows, heads, kv_heads, head_dim, n_groups, max_group, max_shared, max_own)
+    if part_o.numel() < n_rows * heads * parts * head_dim or part_ml.numel() < n_rows * heads * parts * 2:
+        raise KernelArgumentError(f"attention_decode_shared: the scratch for {parts} parts is too small")
+    _check(library().imparo_attention_decode_shared(
+        _dev(q, "q"), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _dev(part_o, "partial outputs", torch.float32),
+        _dev(part_ml, "partial sums", torch.float32), _dev(rows, "decode rows", torch.int32), n_rows,
+        _dev(group_start, "group_start", torch.int32), n_groups, _dev(shared, "shared keys", torch.int32, (n_groups,)),
+        _dev(seg_start, "seg_start", torch.int32), _dev(positions, "positions", torch.int32, (n,)),
+        _dev(block_table, "block table", torch.int32), block_table.shape[1], page_size, heads, kv_heads, head_dim, n_pages,
+        float(scale), int(window or 0), int(max_shared), int(max_own), int(max_group), _stream()), "attention_decode_shared")
+    return out
+
+
 def attention_decode_qkv_takes(head_dim: int, n_freq: int) -> bool:
     """Whether attention_decode_qkv takes heads of this size with this many rotated pairs."""
     return bool(library().imparo_attention_decode_qkv_takes(int(head_dim), int(n_freq)))
@@ -827,13 +917,34 @@ def argmax_rows(logits: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     return out
 
 
+PICK_MAX_VOCAB = 1 << 19          # logits a row that the filtered picks take
+
+
 def sample_rows(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tensor,
-                out: torch.Tensor) -> torch.Tensor:
+                out: torch.Tensor, top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                min_p: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[r]: the first token, in the order of indices, whose running probability under softmax(logits[r] / temperature[r])
+    passes uniform[r]; a temperature of 0 or less takes the largest logit (the first of equal ones).
+
+    Filters, one value a row each, leave out tokens first; in the order "larger logit, then smaller index": `top_k` (int32; 0:
+    off) keeps the first top_k, `top_p` (float32; 1: off) of those the fewest first ones that hold top_p of their probability, the
+    likeliest at least, `min_p` (float32; 0: off) of those the ones with at least min_p of the likeliest one's probability. A row whose
+    filters are all off picks as without them; a filtered row is not given a token below 2^-44 of the likeliest one's
+    probability. A uniform of 1 or more takes the last token that is left. NaN logits are never picked, and an infinite one is
+    picked at once. Rows of at most PICK_MAX_VOCAB logits are filtered."""
     n, vocab = logits.shape
-    _check(library().imparo_sample_rows(
-        _dev(logits, "logits", torch.float32), _dev(temperature, "temperature", torch.float32, (n,)),
-        _dev(uniform, "uniform", torch.float32, (n,)), _dev(out, "picks", torch.int32, (n,)),
-        n, vocab, _stream()), "sample_rows")
+    args = (_dev(logits, "logits", torch.float32), _dev(temperature, "temperature", torch.float32, (n,)),
+            _dev(uniform, "uniform", torch.float32, (n,)))
+    picks = _dev(out, "picks", torch.int32, (n,))
+    if top_k is None and top_p is None and min_p is None:
+        _check(library().imparo_sample_rows(*args, picks, n, vocab, _stream()), "sample_rows")
+        return out
+    _here(logits, "logits")
+    if vocab > PICK_MAX_VOCAB:
+        raise KernelArgumentError(f"sample_rows: rows of {vocab} logits are not filtered, at most {PICK_MAX_VOCAB} are")
+    _check(library().imparo_pick_rows(
+        *args, _dev(top_k, "top_k", torch.int32, (n,)), _dev(top_p, "top_p", torch.float32, (n,)),
+        _dev(min_p, "min_p", torch.float32, (n,)), picks, n, vocab, _stream()), "sample_rows")
     return out
 
 

@@ -1,0 +1,219 @@
+"""Decode attention of rows that share a prefix against the plain form in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import plain_continuations as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def ops():
+    from imparo_amd.kernels import ops as o
+    return o
+
+
+def ints(a):
+    return torch.tensor(np.asarray(a, dtype=np.int32), device=DEV)
+
+
+class Batch:
+    """Groups of (shared keys, [keys behind them, row by row]); rows in no group as (None, [keys]). Pages in no order, everything
+    that no row sees poisoned with NaN, one row of tokens that is not listed, the list in no order of tokens."""
+
+    def __init__(self, groups, heads, kv, dim, page, seed=0, spread=1.5):
+        rng = np.random.default_rng(seed)
+        g = torch.Generator().manual_seed(seed)
+        self.page, self.heads = page, heads
+        total = sum(-(-(s or 0) // page) + sum(-(-((s or 0) + b) // page) + 1 for b in own) for s, own in groups) + 3
+        free = iter(rng.permutation(total).tolist())
+        nan = float("nan")
+        self.k = torch.full((total, kv, page, dim), nan, dtype=torch.bfloat16)
+        self.v = torch.full((total, kv, dim, page), nan, dtype=torch.bfloat16)
+
+        def fill(p, upto):
+            self.k[p, :, :upto] = torch.randn(kv, upto, dim, generator=g).to(torch.bfloat16)
+            self.v[p, :, :, :upto] = torch.randn(kv, dim, upto, generator=g).to(torch.bfloat16)
+
+        tables, positions, self.group_start, self.shared = [], [], [0], []
+        for shared, own in groups:
+            s = shared or 0
+            whole = [next(free) for _ in range(s // page)]
+            for p in whole:
+                fill(p, page)
+            part = next(free) if s % page else None          # the page the shared keys end in: its own copy for every row
+            if part is not None:
+                fill(part, s % page)
+            for j, b in enumerate(own):
+                table = list(whole)
+                if b < 0:                                      # a row inside the prefix
+                    if part is not None:
+                        table.append(part)
+                elif part is not None:
+                    mine = part if j == 0 else next(free)
+                    if mine != part:
+                        self.k[mine], self.v[mine] = self.k[part], self.v[part]
+                    table.append(mine)
+                if b > 0:
+                    while len(table) * page < s + b:
+                        table.append(next(free))
+                    for key in range(s, s + b):
+                        p = table[key // page]
+                        self.k[p, :, key % page] = torch.randn(kv, dim, generator=g).to(torch.bfloat16)
+                        self.v[p, :, :, key % page] = torch.randn(kv, dim, generator=g).to(torch.bfloat16)
+                tables.append(table)
+                positions.append(s + b - 1)
+            if shared is not None:
+                self.group_start.append(len(tables))
+                self.shared.append(s)
+        self.n = n = len(tables)
+        width = max(len(t) for t in tables) + 1
+        self.order = rng.permutation(n)                       # listed row i is row order[i], its token also order[i]
+        self.tables = [None] * n
+        self.positions = [0] * n
+        for i, r in enumerate(self.order):
+            self.tables[r], self.positions[r] = tables[i], positions[i]
+        self.q = (torch.randn(n + 1, heads, dim, generator=g) * spread).to(torch.bfloat16)
+        self.table = np.full((n + 1, width), -1, dtype=np.int32)
+        for r in range(n):
+            self.table[r, :len(self.tables[r])] = self.tables[r]
+        self.max_shared = max(self.shared, default=0)
+        in_group = {i: s for g, s in enumerate(self.shared) for i in range(self.group_start[g], self.group_start[g + 1])}
+        self.max_own = max(max(positions[i] + 1 - in_group.get(i, 0), 0) for i in range(n))
+        self.max_group = max((b - a for a, b in zip(self.group_start, self.group_start[1:])), default=0)
+        self.scale = dim ** -0.5
+
+    def run(self, window=None, stretch=0, scale=None):
+        n, heads, dim = self.q.shape
+        kv = self.k.shape[1]
+        bounds = dict(max_shared=self.max_shared + stretch, max_own=self.max_own + stretch, max_group=self.max_group + stretch)
+        parts = ops().attention_shared_parts(self.n, heads, kv, dim, len(self.shared), bounds["max_group"], bounds["max_shared"],
+                                             bounds["max_own"])
+        nan = float("nan")
+        out = torch.full((n, heads * dim), 7.0, dtype=torch.bfloat16, device=DEV)
+        part_o = torch.full((self.n, heads, parts, dim), nan, device=DEV)
+        part_ml = torch.full((self.n, heads, parts, 2), nan, device=DEV)
+        back = ops().attention_decode_shared(
+            self.q.to(DEV), self.k.to(DEV), self.v.to(DEV), out, part_o, part_ml, ints(self.order), self.n, ints(self.group_start),
+            ints(self.shared), ints(np.arange(n)), ints(self.positions + [0]), ints(self.table), scale or self.scale, window, **bounds)
+        assert back is out
+        assert torch.equal(out[self.n].cpu(), torch.full((heads * dim,), 7.0, dtype=torch.bfloat16))
+        return out[:self.n].cpu()
+
+    def check(self, window=None, stretch=0, scale=None):
+        got = self.run(window, stretch, scale).double()
+        want, bound = plain.attend(self.q[:self.n], self.k, self.v, self.tables, self.positions, scale or self.scale, window)
+        over = (got - want).abs() - bound
+        assert not got.isnan().any() and bool((over <= 0).all()), (float(over.max()), float((got - want).abs().max()))
+
+
+@pytest.mark.parametrize("dim", [16, 32, 48, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("heads,kv", [(4, 4), (6, 2), (8, 1)])
+def test_heads_of_all_sizes(dim, heads, kv):
+    Batch([(200, [3, 40, 1, 70])], heads, kv, dim, 32, seed=dim).check()
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 256])
+@pytest.mark.parametrize("shared", [1, 15, 16, 31, 33, 64, 127, 128, 129, 300, 512, 700])
+def test_where_the_shared_keys_end(page, shared):
+    Batch([(shared, [1, 2, 31, 33, 64])], 4, 2, 32, page, seed=shared).check()
+
+
+@pytest.mark.parametrize("groups", [
+    [(100, [1])],                                              # one row alone in its group
+    [(0, [5, 1, 300])],                                        # a group that shares nothing
+    [(None, [1, 17, 290])],                                    # rows in no group
+    [(64, [0, 0])],                                            # no keys of their own
+    [(64, [4, 9]), (None, [7]), ],                             # the last rows are in no group
+    [(40, [3] * 9), (333, [1, 2, 70]), (16, [500])],
+    [(257, [1] * 70)],                                         # more queries than a block's tile
+    [(90, [-40, -89, 5, -90])],                                # rows inside the prefix, one that sees nothing
+])
+@pytest.mark.parametrize("stretch", [0, 1000])
+def test_groups(groups, stretch):
+    Batch(groups, 4, 2, 64, 16, seed=5).check(stretch=stretch)
+
+
+@pytest.mark.parametrize("heads,kv", [(32, 1), (33, 1), (48, 1), (70, 2)])
+def test_many_heads_a_kv_head(heads, kv):
+    Batch([(75, [1, 30, 9])], heads, kv, 32, 16, seed=heads).check()
+
+
+@pytest.mark.parametrize("window", [1, 7, 32, 100, 260, 10000])
+def test_windows(window):
+    Batch([(290, [1, 40, 128, 300]), (20, [3, 3])], 4, 2, 64, 32, seed=window).check(window=window)
+
+
+@pytest.mark.parametrize("spread,scale", [(0.0, None), (30.0, None), (1.5, -0.2), (1.5, 1e-3)])
+def test_flat_and_steep_scores(spread, scale):
+    """Queries of zero (all keys alike), scores far apart (the reference of the exponentials moves from tile to tile), and scales of either sign."""
+    Batch([(400, [60, 3, 129])], 4, 2, 64, 32, seed=2, spread=spread).check(scale=scale)
+
+
+def test_a_long_prefix():
+    Batch([(4500, [100, 600, 1])], 4, 2, 64, 64, seed=8).check()
+
+
+def test_agrees_with_attention_of_each_row_by_itself():
+    """The same inputs through the kernel that reads everything a row: both inside the bound of the plain form."""
+    b = Batch([(512, [30, 64, 5, 200])], 8, 2, 64, 64, seed=3)
+    n, heads, dim = b.q.shape
+    split = ops().decode_split()
+    context = max(b.positions) + 1
+    n_splits = -(-context // split)
+    out = torch.zeros(n, heads * dim, dtype=torch.bfloat16, device=DEV)
+    ops().attention_decode(b.q.to(DEV), b.k.to(DEV), b.v.to(DEV), out, torch.empty(b.n * heads * n_splits * dim, device=DEV),
+                           torch.empty(b.n * heads * n_splits * 2, device=DEV), ints(b.order), b.n, ints(np.arange(n)),
+                           ints(b.positions + [0]), ints(b.table), b.scale, None, context)
+    _, bound = plain.attend(b.q[:b.n], b.k, b.v, b.tables, b.positions, b.scale)
+    assert bool(((out[:b.n].cpu().double() - b.run().double()).abs() <= 2 * bound).all())
+
+
+def test_replays_follow_what_changes_on_the_device():
+    b = Batch([(200, [40, 50, 60, 70])], 8, 2, 64, 32, seed=6)
+    n, heads, dim = b.q.shape
+    bounds = dict(max_shared=200, max_own=300, max_group=4)      # (the last replay shares nothing)
+    parts = ops().attention_shared_parts(b.n, heads, 2, dim, 1, 4, 200, 300)
+    out = torch.zeros(n, heads * dim, dtype=torch.bfloat16, device=DEV)
+    part_o, part_ml = torch.empty(b.n, heads, parts, dim, device=DEV), torch.empty(b.n, heads, parts, 2, device=DEV)
+    q, k, v, shared, positions = b.q.to(DEV), b.k.to(DEV), b.v.to(DEV), ints([200]), ints(b.positions + [0])
+    args = (q, k, v, out, part_o, part_ml, ints(b.order), b.n, ints([0, 4]), shared, ints(np.arange(n)), positions, ints(b.table),
+            b.scale, None)
+    ops().attention_decode_shared(*args, **bounds)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops().attention_decode_shared(*args, **bounds)
+    for i, (s, back) in enumerate([(200, 0), (192, 3), (96, 30), (0, 0)]):
+        shared.fill_(s)
+        now = [p - back for p in b.positions]
+        positions.copy_(ints(now + [0]))
+        part_o.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, bound = plain.attend(b.q[:b.n], b.k, b.v, b.tables, now, b.scale)
+        assert bool(((out[:b.n].cpu().double() - want).abs() <= bound).all()), i
+
+
+def test_refusals():
+    b = Batch([(32, [4, 4])], 4, 2, 64, 32, seed=1)
+    n, heads, dim = b.q.shape
+    bad = ops().KernelArgumentError
+    good = dict(q=b.q.to(DEV), k_cache=b.k.to(DEV), v_cache=b.v.to(DEV),
+                out=torch.zeros(n, heads * dim, dtype=torch.bfloat16, device=DEV), part_o=torch.zeros(4096 * 8, device=DEV),
+                part_ml=torch.zeros(4096, device=DEV), rows=ints(b.order), n_rows=2, group_start=ints([0, 2]), shared=ints([32]),
+                seg_start=ints(np.arange(n)), positions=ints(b.positions + [0]), block_table=ints(b.table), scale=0.1, window=None,
+                max_shared=32, max_own=8, max_group=2)
+    ops().attention_decode_shared(**good)
+    for name, value in [("q", good["q"].float()), ("k_cache", good["k_cache"].float()), ("out", good["out"][:1]),
+                        ("v_cache", good["v_cache"].transpose(2, 3)), ("n_rows", 3), ("n_rows", -1), ("window", 0), ("window", -4),
+                        ("group_start", ints([])), ("shared", ints([1, 2])), ("block_table", ints(b.table)[:1]),
+                        ("positions", ints([0])), ("part_o", torch.zeros(16, device=DEV)), ("part_ml", torch.zeros(4, device=DEV)),
+                        ("max_own", -1), ("max_shared", (1 << 30) + 1), ("rows", ints(b.order).long()), ("q", good["q"].cpu()),
+                        ("part_o", torch.zeros(4096 * 8 + 4, device=DEV)[1:])]:
+        with pytest.raises(bad):
+            ops().attention_decode_shared(**{**good, name: value})
+    out = torch.full_like(good["out"], 3.0)
+    ops().attention_decode_shared(**{**good, "out": out, "n_rows": 0})
+    assert bool((out == 3.0).all())
