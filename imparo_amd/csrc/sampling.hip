@@ -268,39 +268,28 @@ extern "C" int imparo_sample_rows(const float* logits, const float* temperature,
 // nearest to w 2^44 (w from a float64 exponential), so sums are exact in any order, over any split, and by atomics. 2^19 logits
 // fill 63 bits. A token below 2^-44 of the likeliest is not drawn: all of those together weigh less than 2^-25, under one
 // step of a 24-bit u.
-// The border is found without sorting: a histogram in LDS, linear in the logit over the range that weighs anything, a scan for the bin
-// where the count (or the weight) is reached, and the same again inside that bin over its keys' bits until one key is left.
-// One block a row, which reads it again for each pass (out of L2).
+// One block a row, and what an instruction a logit costs is what the kernel costs (65,536 logits, 64 lanes a clock: 0.43 us each),
+// so the row is read few times (out of L2 after the first) and little is done a logit. First the largest; then a bound under
+// which nothing is kept, as a number of bins, 2,048 over the 44 octaves that weigh anything: for min-p its own; for top-k the k-th
+// largest of the threads' own maxima, as k logits at least are no smaller; for top-p alone the bin of a histogram of weights where p of them
+// is reached. The tokens above that go into a list, four a thread at most, and border, ties and pick are found in the list alone,
+// by histograms over eight bits of keys or indices at a time, one barrier each (list_find). A row whose kept tokens do not fit the list
+// lists the tokens of the border's bin only and picks in two further passes; if not even those fit, everything is done over
+// the row itself, pass by pass (pick_narrow).
 #define PICK_BINS 2048
-#define PICK_LIST 2048
+#define PICK_BITS 9                // bits of a key or an index that a search in the list settles at a time
+#define PICK_FEW 256               // tokens that are compared with one another instead
+#define PICK_EACH 4                // tokens of the list a thread has at most
 #define PICK_CUT 44
 
 typedef unsigned long long u64;
 
-// the float's place in the order of floats
+// the float's place in the order of floats (-0 and 0 are one), and back
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.f);
     return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-
-// 2^y 2^44 to the nearest integer, y <= 0 (0 below 2^-44.5): 2^f = e^(f ln 2) of the fraction |f| <= 1/2 as its power series, cut where the next
-// term is below 2^-47, then scaled by the exponent and rounded by an addition of 2^52
-__device__ __forceinline__ u64 weight_of(double y) {
-    const double k = rint(y), f = (y - k) * 0.69314718055994530942;
-    double p = fma(f, 1.0 / 39916800.0, 1.0 / 3628800.0);
-    p = fma(f, p, 1.0 / 362880.0);
-    p = fma(f, p, 1.0 / 40320.0);
-    p = fma(f, p, 1.0 / 5040.0);
-    p = fma(f, p, 1.0 / 720.0);
-    p = fma(f, p, 1.0 / 120.0);
-    p = fma(f, p, 1.0 / 24.0);
-    p = fma(f, p, 1.0 / 6.0);
-    p = fma(f, p, 0.5);
-    p = fma(f, p, 1.0);
-    p = fma(f, p, 1.0);
-    const double scaled = __hiloint2double(__double2hiint(p) + (((int)k + PICK_CUT) << 20), __double2loint(p));
-    return y < -(PICK_CUT + 0.5) ? 0 : (u64)__double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
-}
+__device__ __forceinline__ float float_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
 template <int N>
 __device__ __forceinline__ u64 lane_xor_u64(u64 v) {
@@ -315,35 +304,74 @@ __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
     v += lane_xor_u64<32>(v);
     return v;
 }
-__device__ __forceinline__ u64 wave_scan_u64(u64 v) {             // the sum over the lanes up to and with this one
-    const int lane = threadIdx.x & (WAVE - 1);
-#pragma unroll
-    for (int n = 1; n < WAVE; n <<= 1) {
-        const u64 below = __shfl_up(v, n, WAVE);
-        if (lane >= n) v += below;
-    }
+// What CTRL moves to this lane, 0 where nothing comes: the steps of a running sum over the lanes
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved(u64 v) {
+    return ((u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false) << 32) |
+           (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, ROWS, 0xf, false));
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {                     // the sum over the lanes up to and with this one
+    v += moved<0x111, 0xf>(v);                                    // row_shr:1, 2, 4, 8
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);                                    // lane 15 of a row of 16 to the next row: rows 1 and 3
+    v += moved<0x143, 0xc>(v);                                    // lane 31 to rows 2 and 3
     return v;
 }
 
 struct PickShared {
     u64 hist[PICK_BINS];
-    uint32_t list[PICK_LIST];
-    u64 waves[16];
-    float tops[16], lows[16];
-    u64 above, inside, total, need;   // of the bin where the sum is reached: what lies above it, what it holds; all there is; what is asked for
-    int bin, n_list;
+    u64 level[2][1 << PICK_BITS];     // used in turn: while one is read the other is cleared
+    float list_x[PICK_EACH * 1024];
+    int list_index[PICK_EACH * 1024];
+    double table[32];                 // 2^(i / 32)
+    u64 waves[16], turns[132];
+    float tops[16];
+    u64 few_ord[PICK_FEW], few_weight[PICK_FEW], few_mass[2][PICK_FEW], few_sum[2];
+    int few_rank[PICK_FEW];
+    u64 above, inside, need;          // of the bin where the sum is reached: what lies above it, what it holds; what is asked for
+    int bin, n_list, cut, reached;
+    uint32_t low;
     uint32_t key_low, key_high;
-    int cut;
+};
+
+// Weights of a row: 2^y 2^44 to the nearest integer, y = (x - top) c1 <= 0, as an integer in a double. y 32 = n + f with n whole, 2^(n / 32)
+// out of a table and an exponent, and 2^(f / 32), |f| <= 1/2, from its power series, cut where the next term is below 2^-48; rounded by
+// an addition of 2^52, whose low bits then are the integer.
+struct PickWeights {
+    double top, c32;
+    const double* table;
+    __device__ __forceinline__ u64 operator()(float x) const {
+        constexpr double MAGIC = 6755399441055744.0, L = 0.69314718055994530942 / 32;
+        const double d = (double)x - top, t = fma(d, c32, MAGIC), f = fma(d, c32, -(t - MAGIC));
+        const int n = __double2loint(t);
+        double p = fma(f, L * L * L * L * L / 120, L * L * L * L / 24);
+        p = fma(f, p, L * L * L / 6);
+        p = fma(f, p, L * L / 2);
+        p = fma(f, p, L);
+        p = fma(f, p, 1.0);
+        const double v = ldexp(p * table[n & 31], (n >> 5) + PICK_CUT) + 4503599627370496.0;
+        const u64 whole = (u64)__double_as_longlong(v) & 0xFFFFFFFFFFFFFull;
+        return d * c32 >= -32.0 * PICK_CUT - 16.0 ? whole : 0;
+    }
+    __device__ __forceinline__ double octaves(float x) const { return ((double)x - top) * c32 * 0.03125; }
 };
 
 // The bin of sh.hist where the running sum reaches what is asked for: `need`, or for share >= 0 that share of all. Leaves bin,
-// above, inside, total and need in LDS; every thread calls, behind and ahead of a barrier of its own.
+// above, inside and need in LDS; bin is -1 where the sum is never reached. Every thread calls, behind and ahead of a barrier of its own.
 __device__ __forceinline__ void pick_bin(PickShared& sh, u64 need, double share) {
     const int threads = blockDim.x, per = PICK_BINS / threads, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     u64 mine = 0;
     for (int i = 0; i < per; ++i) mine += sh.hist[tid * per + i];
-    const u64 upto = wave_scan_u64(mine);
+    const u64 upto = wave_scan(mine);
     if (lane == WAVE - 1) sh.waves[wave] = upto;
+    if (tid == 0) sh.bin = -1;
     __syncthreads();
     u64 before = 0, total = 0;
     for (int w = 0; w < threads / WAVE; ++w) {
@@ -363,7 +391,6 @@ __device__ __forceinline__ void pick_bin(PickShared& sh, u64 need, double share)
         sh.bin = b;
         sh.above = at;
         sh.inside = v;
-        sh.total = total;
         sh.need = need;
     }
     __syncthreads();
@@ -371,39 +398,47 @@ __device__ __forceinline__ void pick_bin(PickShared& sh, u64 need, double share)
 
 // A row's logits, lane by lane: wave w has the values of its own run, 256 a turn, four neighbours a lane. What stands in front of
 // the row or behind it inside the 16 aligned bytes that hold its first or last value is read with them (the same 16 bytes of
-// memory, so it is there) and counts as -inf, as NaN does.
-#define PICK_DEEP 8
+// memory, so it is there) and counts as NaN, which every comparison passes over.
 struct PickRow {
     const float4* base;
     int skew, vocab, turns, first;      // first: index in the row of this lane's first value in turn 0
+    int wave_first;                     // the same of the wave's first lane
 
     __device__ __forceinline__ void open(const float* row, int n) {
         vocab = n;
         skew = (int)(((uintptr_t)row & 15) >> 2);
         base = reinterpret_cast<const float4*>(row - skew);
-        const int waves = blockDim.x / WAVE, lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+        const int waves = blockDim.x / WAVE, lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
         turns = (vocab + skew + 4 * WAVE * waves - 1) / (4 * WAVE * waves);
-        first = wave * turns * 4 * WAVE + 4 * lane - skew;
+        of_wave(wave);
     }
-    // f(values, index of the first of the four), turn after turn, the loads of PICK_DEEP turns in flight
-    template <typename F>
+    __device__ __forceinline__ void of_wave(int wave) {
+        wave_first = wave * turns * 4 * WAVE - skew;
+        first = wave_first + 4 * ((int)threadIdx.x & (WAVE - 1));
+    }
+    __device__ __forceinline__ float4 load(int c) const { return base[min(max(first + skew + c * 4 * WAVE, 0), vocab + skew - 1) >> 2]; }
+    __device__ __forceinline__ void values(float (&x)[4], const float4& v, int c) const {
+        const int i = first + c * 4 * WAVE, w = wave_first + c * 4 * WAVE;
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        if (w < 0 || w + 4 * WAVE > vocab) {                      // (the wave's turn reaches past an end of the row)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = i + j >= 0 && i + j < vocab ? x[j] : __builtin_nanf("");
+        }
+    }
+    // f(values, index of the first of the four), turn after turn, the loads of DEEP turns in flight. Code that a block runs through once
+    // comes out of memory too: long bodies are better off in a loop than written out many times.
+    template <int DEEP = 4, typename F>
     __device__ __forceinline__ void each(F f) const {
-        for (int c0 = 0; c0 < turns; c0 += PICK_DEEP) {
-            float4 v[PICK_DEEP];
+        for (int c0 = 0; c0 < turns; c0 += DEEP) {
+            float4 v[DEEP];
 #pragma unroll
-            for (int c = 0; c < PICK_DEEP; ++c)
-                v[c] = base[min(max(first + skew + (c0 + c) * 4 * WAVE, 0), vocab + skew - 1) >> 2];
+            for (int c = 0; c < DEEP; ++c) v[c] = load(c0 + c);
 #pragma unroll
-            for (int c = 0; c < PICK_DEEP; ++c) {
+            for (int c = 0; c < DEEP; ++c) {
                 if (c0 + c >= turns) break;
-                const int i = first + (c0 + c) * 4 * WAVE;
-                float x[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const bool on = i + j >= 0 && i + j < vocab && x[j] == x[j];
-                    x[j] = on ? x[j] + 0.f : -INFINITY;          // (+ 0: -0 and 0 are one value)
-                }
-                f(x, i);
+                float x[4];
+                values(x, v[c], c0 + c);
+                f(x, first + (c0 + c) * 4 * WAVE);
             }
         }
     }
@@ -416,68 +451,218 @@ struct PickSet {
     __device__ __forceinline__ bool has(uint32_t k, int index) const { return k > key || (k == key && index <= cut); }
 };
 
-// Narrows `set` to the beginning of its order where the count (COUNT) reaches `need`, or the weights the share `share` of theirs.
+// ---- in the list: a thread's tokens, and for the search at hand what each counts and where it stands in the order
+struct PickList {
+    float x[PICK_EACH];
+    int index[PICK_EACH];
+    u64 weight[PICK_EACH], counts[PICK_EACH];
+    uint32_t ord[PICK_EACH];
+    int n, turn;                       // tokens of this thread; the histogram that is next in turn
+
+    __device__ __forceinline__ void take(const PickShared& sh, const PickWeights& weights, int threads) {
+        const int all = sh.n_list;
+        n = 0;
+#pragma unroll
+        for (int e = 0; e < PICK_EACH; ++e) {
+            const int at = e * threads + (int)threadIdx.x;
+            if (e * threads >= all) break;
+            if (at < all) {
+                x[e] = sh.list_x[at];
+                index[e] = sh.list_index[at];
+                weight[e] = weights(x[e]);
+                n = e + 1;
+            }
+        }
+    }
+};
+
+// Where, among the list's tokens and in the order of `ord` (whole numbers from low to high, the smallest first), the running sum of `counts`
+// reaches `need`, or of their sum the part that `asked` says (asked(sum)): sets ord, above and inside of the one that is passed at; false where it is never
+// reached. PICK_BITS at a time: a histogram by atomics, and one wave adds its bins up (all of them for themselves would take four times as
+// long: a SIMD has four of them).
+struct Found {
+    uint32_t ord;
+    u64 above, inside, need;
+};
+template <typename A>
+__device__ __forceinline__ bool list_find(PickShared& sh, PickList& list, uint32_t low, uint32_t high, Found& found, A asked) {
+    constexpr int BINS = 1 << PICK_BITS, PER = BINS / WAVE;
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1);
+    u64 above = 0, need = 0;
+    for (bool first = true;; first = false) {
+        const int bits = low == high ? 0 : 32 - __clz((int)(high - low)), shift = max(0, bits - PICK_BITS);
+        u64* hist = sh.level[list.turn];
+        list.turn ^= 1;
+#pragma unroll
+        for (int e = 0; e < PICK_EACH; ++e)
+            if (e < list.n && list.counts[e] && list.ord[e] >= low && list.ord[e] <= high)
+                atomicAdd(&hist[(list.ord[e] - low) >> shift], list.counts[e]);
+        __syncthreads();
+        if (tid >= WAVE) {
+            for (int b = tid - WAVE; b < BINS; b += (int)blockDim.x - WAVE) sh.level[list.turn][b] = 0;
+        } else {
+            u64 bin[PER], mine = 0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                bin[i] = hist[PER * lane + i];
+                mine += bin[i];
+            }
+            const u64 upto = wave_scan(mine);
+            if (first) need = asked(((u64)(uint32_t)__builtin_amdgcn_readlane((int)(upto >> 32), WAVE - 1) << 32) |
+                                    (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)upto, WAVE - 1));
+            u64 at = upto - mine + above;
+            const bool here = at < need && need <= at + mine;
+            if (lane == 0 && !__any(here)) sh.reached = 0;
+            if (here) {
+                int b = 0;
+                u64 inside = bin[0];
+#pragma unroll
+                for (int i = 0; i < PER - 1; ++i)
+                    if (b == i && at + bin[i] < need) {
+                        at += bin[i];
+                        b = i + 1;
+                        inside = bin[i + 1];
+                    }
+                sh.reached = 1;
+                sh.above = at;
+                sh.inside = inside;
+                sh.need = need;
+                sh.low = low + ((uint32_t)(PER * lane + b) << shift);
+            }
+        }
+        __syncthreads();
+        if (!sh.reached) return false;
+        low = sh.low;
+        above = sh.above;
+        need = sh.need;
+        if (shift == 0) break;
+        high = high - low > (1u << shift) - 1 ? low + ((1u << shift) - 1) : high;
+    }
+    found = Found{low, above, sh.inside, need};
+    return true;
+}
+// The running sum at which a uniform number picks: the first whole number above u times the sum, and no more than the sum (at which the last
+// token is reached). A NaN counts as 0.
+__device__ __forceinline__ u64 passed_at(float u, u64 total) {
+    return min((u64)fmin(fmax((double)u * (double)total, 0.0), (double)total), total - 1) + 1;
+}
+
+// The whole choice in a list of at most PICK_FEW tokens: every token is compared with every other one. How many stand before it in the order, and
+// what they weigh, says whether it is kept; what the kept ones of smaller indices weigh, whether it is picked. Two rounds of compares (128
+// tokens: 0.2 us of them each) and five barriers, where the searches bit by bit take up to a dozen rounds behind one another.
+template <int THREADS>
+__device__ __forceinline__ void pick_few(PickShared& sh, const PickWeights& weights, int k, double share, bool by_k, bool by_p, u64 need_p, double floor_y,
+                                         float u, int32_t* out) {
+    const int tid = threadIdx.x, n = sh.n_list;
+    const int bits = n <= WAVE ? 6 : 32 - __clz(n - 1);           // entries a row of threads: whole waves, so that a wave compares with one token at a time
+    const int i = tid & ((1 << bits) - 1), part = tid >> bits, parts = THREADS >> bits;
+    u64 weight = 0;
+    int index = 0;
+    bool kept = false;
+    if (tid < n) {
+        const float x = sh.list_x[tid];
+        index = sh.list_index[tid];
+        weight = weights(x);
+        kept = weights.octaves(x) >= floor_y;
+        sh.few_ord[tid] = (u64)~key_of(x) << 32 | (uint32_t)index;
+        sh.few_weight[tid] = weight;
+        sh.few_mass[0][tid] = sh.few_mass[1][tid] = 0;
+        sh.few_rank[tid] = 0;
+    }
+    if (tid < 2) sh.few_sum[tid] = 0;
+    __syncthreads();
+    u64 mass = 0;
+    int rank = 0;
+    const u64 ord = sh.few_ord[i];                                // (past the list: not used)
+    for (int j = part; j < n; j += parts) {
+        const u64 w = sh.few_weight[j];
+        const bool before = sh.few_ord[j] < ord;
+        rank += before;
+        mass += before ? w : 0;
+    }
+    if (i < n) {
+        atomicAdd(&sh.few_mass[0][i], mass);
+        atomicAdd(&sh.few_rank[i], rank);
+    }
+    __syncthreads();
+    if (tid < n) {
+        mass = sh.few_mass[0][tid];
+        rank = sh.few_rank[tid];
+        kept = kept && (!by_k || rank < k);
+        if (by_k && by_p && rank == min(k, n) - 1) sh.few_sum[0] = mass + weight;
+    }
+    if (by_k && by_p) {
+        __syncthreads();
+        need_p = max((u64)1, (u64)ceil(share * (double)sh.few_sum[0]));
+    }
+    if (by_p) kept = kept && mass < need_p;
+    weight = kept ? weight : 0;
+    if (tid < PICK_FEW) {                                         // (whole waves)
+        if (tid < n) sh.few_weight[tid] = weight;
+        const u64 sum = wave_sum_u64(tid < n ? weight : 0);
+        if ((tid & (WAVE - 1)) == 0) atomicAdd(&sh.few_sum[1], sum);
+    }
+    __syncthreads();
+    mass = 0;
+    for (int j = part; j < n; j += parts) mass += (uint32_t)sh.few_ord[j] < (uint32_t)ord ? sh.few_weight[j] : 0;
+    if (i < n) atomicAdd(&sh.few_mass[1][i], mass);
+    __syncthreads();
+    if (tid < n && weight) {
+        const u64 before = sh.few_mass[1][tid], target = passed_at(u, sh.few_sum[1]) - 1;
+        if (before <= target && target < before + weight) *out = index;
+    }
+}
+
+// What is left to do in the list, in this order; the searches for ties only where not all of them stay
+enum { PICK_K, PICK_K_TIES, PICK_P, PICK_P_TIES, PICK_DRAW };
+
+// ---- in the row: the same, a pass over the row for each step
 template <bool COUNT>
 __device__ __forceinline__ void pick_narrow(PickShared& sh, const PickRow& row, PickSet& set, float top, float bin_scale,
-                                            float reach, float c1f, double c1, u64 need, double share) {
+                                            const PickWeights& weights, u64 need, double share) {
     const int tid = threadIdx.x, threads = blockDim.x;
-    auto weight = [&](float x) { return COUNT ? (u64)1 : weight_of(((double)x - (double)top) * c1); };
-    auto bin_of = [&](float x) { return (int)fminf((top - x) * bin_scale, (float)(PICK_BINS - 1)); };
+    auto weight = [&](float x) { return COUNT ? (u64)1 : weights(x); };
+    auto place = [&](float x) { return (top - x) * bin_scale; };
+    __syncthreads();
     for (int b = tid; b < PICK_BINS; b += threads) sh.hist[b] = 0;
     if (tid == 0) {
-        sh.n_list = 0;
         sh.key_low = 0xFFFFFFFFu;
         sh.key_high = 0;
-        sh.total = 0;
     }
     __syncthreads();
     row.each([&](const float (&x)[4], int index) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (x[j] >= reach && set.has(key_of(x[j]), index + j)) atomicAdd(&sh.hist[bin_of(x[j])], weight(x[j]));
+            if (place(x[j]) < (float)PICK_BINS && set.has(key_of(x[j]), index + j)) atomicAdd(&sh.hist[(int)place(x[j])], weight(x[j]));
     });
     __syncthreads();
     pick_bin(sh, need, share);
-    if (sh.total == 0) return;                                    // fewer than are asked for: all stay
-    u64 above = sh.above;
+    if (sh.bin < 0) return;                                       // fewer than are asked for: all stay
+    u64 above = sh.above, inside = sh.inside;
     need = sh.need;
     const int bin = sh.bin;
     row.each([&](const float (&x)[4], int index) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (!(x[j] >= reach) || bin_of(x[j]) != bin) continue;
-            const uint32_t k = key_of(x[j]);
-            if (!set.has(k, index + j)) continue;
-            const int at = atomicAdd(&sh.n_list, 1);
-            if (at < PICK_LIST) sh.list[at] = k;
-            atomicMin(&sh.key_low, k);
-            atomicMax(&sh.key_high, k);
+            if (!(place(x[j]) < (float)PICK_BINS) || (int)place(x[j]) != bin || !set.has(key_of(x[j]), index + j)) continue;
+            atomicMin(&sh.key_low, key_of(x[j]));
+            atomicMax(&sh.key_high, key_of(x[j]));
         }
     });
     __syncthreads();
-    const int n_list = sh.n_list;
     uint32_t low = sh.key_low, high = sh.key_high;
-    u64 inside = sh.inside;
     while (low != high) {                                         // (at most three times: 11 bits of at most 32 each)
         const int bits = 32 - __clz((int)(high - low)), shift = max(0, bits - 11);
         __syncthreads();
         for (int b = tid; b < PICK_BINS; b += threads) sh.hist[b] = 0;
         __syncthreads();
-        auto float_of = [](uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); };
-        if (n_list <= PICK_LIST) {
-            for (int i = tid; i < n_list; i += threads) {
-                const uint32_t k = sh.list[i];
-                if (k >= low && k <= high) atomicAdd(&sh.hist[(high - k) >> shift], weight(float_of(k)));
-            }
-        } else {
-            row.each([&](const float (&x)[4], int index) {
+        row.each([&](const float (&x)[4], int index) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t k = key_of(x[j]);
-                    if (x[j] >= reach && k >= low && k <= high && set.has(k, index + j)) atomicAdd(&sh.hist[(high - k) >> shift], weight(x[j]));
-                }
-            });
-        }
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t k = key_of(x[j]);
+                if (x[j] == x[j] && k >= low && k <= high && set.has(k, index + j)) atomicAdd(&sh.hist[(high - k) >> shift], weight(x[j]));
+            }
+        });
         __syncthreads();
         pick_bin(sh, need - above, -1.0);
         above += sh.above;
@@ -486,21 +671,18 @@ __device__ __forceinline__ void pick_narrow(PickShared& sh, const PickRow& row, 
         low = high - low > (1u << shift) - 1 ? high - ((1u << shift) - 1) : low;
     }
     // one key is left: so many of its tokens, in the order of their indices, reach what is asked for
-    const u64 each = weight(__uint_as_float(high & 0x80000000u ? high ^ 0x80000000u : ~high));
-    const u64 ties = (need - above + each - 1) / each;
-    const PickSet old = set;
+    const u64 each = weight(float_of(high)), ties = (need - above + each - 1) / each;
+    set.cut = high == set.key ? set.cut : INT_MAX;
     set.key = high;
-    set.cut = INT_MAX;
-    if (ties * each >= inside) {                                  // all of them
-        if (high == old.key) set.cut = old.cut;
-        return;
-    }
+    if (ties * each >= inside) return;                            // all of them
     const int lane = tid & (WAVE - 1), wave = tid / WAVE;
+    const float tie = float_of(high);
     u64 mine = 0;
-    row.each([&](const float (&x)[4], int index) {
+    row.each([&](const float (&x)[4], int) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mine += __popcll(__ballot(x[j] >= reach && key_of(x[j]) == high));
+        for (int j = 0; j < 4; ++j) mine += __popcll(__ballot(x[j] == tie));
     });
+    __syncthreads();
     if (lane == 0) sh.waves[wave] = mine;
     __syncthreads();
     u64 before = 0;
@@ -510,18 +692,69 @@ __device__ __forceinline__ void pick_narrow(PickShared& sh, const PickRow& row, 
             u64 ahead = before;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const bool on = x[j] >= reach && key_of(x[j]) == high;
-                const u64 who = __ballot(on);
+                const u64 who = __ballot(x[j] == tie);
                 ahead += __popcll(who & ((1ull << lane) - 1));
                 before += __popcll(who);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (x[j] >= reach && key_of(x[j]) == high && ++ahead == ties) sh.cut = index + j;
+                if (x[j] == tie && ++ahead == ties) sh.cut = index + j;
         });
     }
     __syncthreads();
     set.cut = sh.cut;
+}
+
+// The pick out of the row, for what `kept` says of a logit and its index: sums over the waves' runs, then all waves take the turns of the run
+// where u falls, then a wave the turn.
+template <typename K>
+__device__ __forceinline__ void pick_from_row(PickShared& sh, PickRow row, float u, const PickWeights& weights, int32_t* out, K kept) {
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE, waves = blockDim.x / WAVE;
+    u64 mine = 0;
+    row.each([&](const float (&x)[4], int index) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (kept(x[j], index + j)) mine += weights(x[j]);
+    });
+    const u64 of_wave = wave_sum_u64(mine);
+    __syncthreads();
+    if (lane == 0) sh.waves[wave] = of_wave;
+    __syncthreads();
+    u64 total = 0;
+    for (int w = 0; w < waves; ++w) total += sh.waves[w];
+    const u64 target = passed_at(u, total) - 1;
+    u64 before = 0;
+    int run = 0;
+    while (before + sh.waves[run] <= target) before += sh.waves[run++];
+    row.of_wave(run);
+    auto four_of = [&](int c, u64 (&w)[4]) {
+        float x[4];
+        row.values(x, row.load(c), c);
+        u64 sum = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            w[j] = kept(x[j], row.first + c * 4 * WAVE + j) ? weights(x[j]) : 0;
+            sum += w[j];
+        }
+        return sum;
+    };
+    for (int c = wave; c < row.turns; c += waves) {
+        u64 w[4];
+        const u64 sum = wave_sum_u64(four_of(c, w));
+        if (lane == 0) sh.turns[c] = sum;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    int c = 0;
+    while (before + sh.turns[c] <= target) before += sh.turns[c++];
+    u64 w[4];
+    const u64 four = four_of(c, w), upto = wave_scan(four), past = __ballot(before + upto > target);
+    if (lane == __ffsll((long long)past) - 1) {
+        u64 at = before + upto - four;
+        int j = 0;
+        while (j < 3 && at + w[j] <= target) at += w[j++];
+        *out = row.first + c * 4 * WAVE + j;
+    }
 }
 
 template <int THREADS>
@@ -531,6 +764,7 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
     int32_t* __restrict__ out, int vocab) {
     __shared__ PickShared sh;
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    constexpr int WAVES = THREADS / WAVE, ROOM = PICK_EACH * THREADS;
     const float* row_at = logits + (size_t)r * vocab;
     const float temp = temperature[r], u = uniform[r];
     const int k = top_k ? top_k[r] : 0;
@@ -542,101 +776,167 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
     }
     PickRow row;
     row.open(row_at, vocab);
-    float top = -INFINITY, low = INFINITY;
-    row.each([&](const float (&x)[4], int) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            top = fmaxf(top, x[j]);
-            low = fminf(low, x[j] > -INFINITY ? x[j] : INFINITY);
-        }
-    });
-    top = wave_max(top);
-    low = -wave_max(-low);
-    if (lane == 0) {
-        sh.tops[wave] = top;
-        sh.lows[wave] = low;
-    }
+    float own_top = -INFINITY;                                    // the largest of this thread's
+    auto largest = [&](const float (&x)[4]) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); };
+    if (tid < 32) sh.table[tid] = exp2((double)tid * 0.03125);
+    for (int b = tid; b < PICK_BINS; b += THREADS) sh.hist[b] = 0;
+    for (int b = tid; b < 2 << PICK_BITS; b += THREADS) (&sh.level[0][0])[b] = 0;
+    if (tid == 0) sh.n_list = 0;
+    row.each<8>([&](const float (&x)[4], int) { own_top = fmaxf(own_top, largest(x)); });
+    float top = wave_max(own_top);
+    if (lane == 0) sh.tops[wave] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < THREADS / WAVE; ++w) {
-        top = fmaxf(top, sh.tops[w]);
-        low = fminf(low, sh.lows[w]);
-    }
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sh.tops[w]);
     if (!(top < INFINITY) || !(top > -INFINITY)) {                // an infinite logit takes it, or there is none to take
         sample_row(row_at, 0.f, u, out + r, vocab);
         return;
     }
     const double c1 = 1.44269504088896340736 / (double)temp;
-    const float c1f = fminf((float)c1, 3.0e38f);
-    // logits below `reach` weigh nothing; a token that min-p takes out is not looked at again either, as every smaller one goes too
+    const PickWeights weights{(double)top, 32.0 * c1, sh.table};
     const double floor_y = by_m ? fmax(-(double)PICK_CUT, log2((double)fminf(mp, 1.f))) : -(double)PICK_CUT;
-    const float span = fminf(top - low, (float)PICK_CUT / c1f);
-    const float reach = fmaxf(low, top - (float)PICK_CUT / c1f);
-    const float bin_scale = span > 1e-30f && span < 1e30f ? (float)PICK_BINS * 0.99999f / span : 0.f;
-    PickSet set{0u, INT_MAX};
-    if (by_k) pick_narrow<true>(sh, row, set, top, bin_scale, reach, c1f, c1, (u64)k, -1.0);
-    __syncthreads();
-    if (by_p) pick_narrow<false>(sh, row, set, top, bin_scale, reach, c1f, c1, 0, (double)fmaxf(p, 0.f));
-    __syncthreads();
+    // bins an octave, and a unit of the logit: a logit d below the top is in bin d bin_scale
+    constexpr float BINS_AN_OCTAVE = (float)PICK_BINS / PICK_CUT;
+    const float bin_scale = BINS_AN_OCTAVE * fminf((float)c1, 1.0e36f);
+    auto place = [&](float x) { return (top - x) * bin_scale; };
 
-    // ---- the pick: sums over the waves' runs, then inside the run where u falls
-    auto kept = [&](float x, int index) {
-        return x >= reach && set.has(key_of(x), index) && ((double)x - (double)top) * c1 >= floor_y;
-    };
-    u64 mine = 0;
-    int last = -1;
-    row.each([&](const float (&x)[4], int index) {
+    // ---- how far down the list has to reach: `limit`, a number of bins
+    float limit = (float)PICK_BINS;
+    const double share = (double)fmaxf(p, 0.f);
+    u64 need_p = 0;
+    if (by_k) {
+        if (k <= THREADS / 2) {
+            // the k-th largest of the threads' maxima: so many logits at least are no smaller, and not many more
+            if (place(own_top) < (float)PICK_BINS) atomicAdd(&sh.hist[(int)place(own_top)], (u64)1);
+            __syncthreads();
+            pick_bin(sh, (u64)k, -1.0);
+            if (sh.bin >= 0) limit = (float)(sh.bin + 1);
+        } else {
+            row.each([&](const float (&x)[4], int) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (kept(x[j], index + j)) {
-                mine += weight_of(((double)x[j] - (double)top) * c1);
-                last = index + j;
-            }
-    });
-    mine = wave_sum_u64(mine);
-    if (lane == 0) sh.waves[wave] = mine;
-    if (tid == 0) sh.cut = -1;
-    __syncthreads();
-    u64 before = 0, total = 0;
-    for (int w = 0; w < THREADS / WAVE; ++w) {
-        before += w < wave ? sh.waves[w] : 0;
-        total += sh.waves[w];
-    }
-    const double want = fmax((double)u * (double)total, 0.0);     // (a NaN is 0)
-    if (!(want < (double)total)) {                                // u of 1: the last token that is kept
-        if (last >= 0) atomicMax(&sh.cut, last);
-        __syncthreads();
-        if (tid == 0) out[r] = sh.cut;
-        return;
-    }
-    const u64 target = min((u64)want, total - 1);
-    if (before <= target && target < before + mine) {
-        int found = -1;
-        row.each([&](const float (&x)[4], int index) {
-            if (found >= 0) return;
-            u64 w[4], four = 0;
+                for (int j = 0; j < 4; ++j)
+                    if (place(x[j]) < (float)PICK_BINS) atomicAdd(&sh.hist[(int)place(x[j])], (u64)1);
+            });
+            __syncthreads();
+            pick_bin(sh, (u64)k, -1.0);
+            if (sh.bin >= 0) limit = (float)(sh.bin + 1);
+        }
+    } else if (by_p) {
+        row.each([&](const float (&x)[4], int) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                w[j] = kept(x[j], index + j) ? weight_of(((double)x[j] - (double)top) * c1) : 0;
-                four += w[j];
+                const float at = place(x[j]);
+                if (at < (float)PICK_BINS) atomicAdd(&sh.hist[(int)at], weights(x[j]));
             }
-            if (!__any(four != 0)) return;
-            const u64 upto = wave_scan_u64(four);
-            const u64 past = __ballot(before + upto > target);
-            if (past) {
-                u64 at = before + upto - four;
-                int pick = -1;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    at += w[j];
-                    if (pick < 0 && at > target) pick = index + j;
-                }
-                found = __shfl(pick, __ffsll((long long)past) - 1, WAVE);
-            }
-            before += __shfl(upto, WAVE - 1, WAVE);
         });
-        if (lane == 0) out[r] = found;
+        __syncthreads();
+        pick_bin(sh, 0, share);
+        need_p = sh.need;
+        limit = (float)(sh.bin + 1);
     }
+    // (a token that min-p takes out need not be listed, unless top-p asks for the sum of the k largest)
+    if (by_m && !(by_k && by_p)) limit = fminf(limit, (float)(-floor_y * (double)BINS_AN_OCTAVE) * 1.0001f + 0.01f);
+
+    // ---- the list
+    auto enlist = [&](const float (&x)[4], int index, float from, float to) {
+        if (place(largest(x)) < to) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (place(x[j]) < to && place(x[j]) >= from) {
+                    const int at = atomicAdd(&sh.n_list, 1);
+                    if (at < ROOM) {
+                        sh.list_x[at] = x[j];
+                        sh.list_index[at] = index + j;
+                    }
+                }
+        }
+    };
+    row.each([&](const float (&x)[4], int index) { enlist(x, index, -1.f, limit); });
+    __syncthreads();
+    PickSet set{0u, INT_MAX};
+    const uint32_t key_high = key_of(top);
+    auto key_under = [&](float bins) { return key_of(top - bins / bin_scale * 1.0001f - fabsf(top) * 1.0e-5f); };   // (no lower place's key is above)
+    if (sh.n_list <= PICK_FEW) {
+        pick_few<THREADS>(sh, weights, k, share, by_k, by_p, need_p, floor_y, u, out + r);
+        return;
+    }
+    PickList list;
+    list.turn = 0;
+    uint32_t key_low = key_under(limit);
+    int stage = by_k ? PICK_K : by_p ? PICK_P : PICK_DRAW;
+    bool from_row = sh.n_list > ROOM;                             // too many for the list: the pick is made out of the row
+    if (from_row) {
+        bool border = false;
+        if (by_p && !by_k) {                                      // the tokens of the border's bin, and what is asked for beyond what lies above
+            const float bin = (float)sh.bin;
+            need_p -= sh.above;
+            __syncthreads();
+            if (tid == 0) sh.n_list = 0;
+            __syncthreads();
+            row.each([&](const float (&x)[4], int index) { enlist(x, index, bin, bin + 1.f); });
+            __syncthreads();
+            border = sh.n_list <= ROOM;
+            key_low = key_under(bin + 1.f);
+            if (!border) need_p += sh.above;
+        }
+        if (!border) {                                            // over the row itself
+            if (by_k) pick_narrow<true>(sh, row, set, top, bin_scale, weights, (u64)k, -1.0);
+            if (by_p) pick_narrow<false>(sh, row, set, top, bin_scale, weights, 0, share);
+            stage = PICK_DRAW;
+        }
+    }
+    if (!from_row || stage != PICK_DRAW) {
+        list.take(sh, weights, THREADS);
+        Found at;
+        int ties_of = 0;                                          // (the search behind the ties)
+        u64 ties = 0;
+        uint32_t tie_key = 0;
+        for (;;) {
+            const bool by_index = stage == PICK_K_TIES || stage == PICK_P_TIES || stage == PICK_DRAW, one_each = stage == PICK_K || stage == PICK_K_TIES;
+#pragma unroll
+            for (int e = 0; e < PICK_EACH; ++e)
+                if (e < list.n) {
+                    const uint32_t key = key_of(list.x[e]);
+                    bool in = set.has(key, list.index[e]);
+                    if (stage == PICK_K_TIES || stage == PICK_P_TIES) in = in && key == tie_key;
+                    if (stage == PICK_DRAW) in = in && weights.octaves(list.x[e]) >= floor_y;
+                    list.counts[e] = !in ? 0 : one_each ? 1 : list.weight[e];
+                    list.ord[e] = by_index ? (uint32_t)list.index[e] : ~key;
+                }
+            const bool reached = list_find(sh, list, by_index ? 0u : ~key_high, by_index ? (uint32_t)vocab - 1 : ~key_low, at, [&](u64 sum) {
+                if (stage == PICK_K) return (u64)k;
+                if (stage == PICK_P) return by_k ? max((u64)1, (u64)ceil(share * (double)sum)) : need_p;
+                if (stage == PICK_DRAW) return passed_at(u, sum);
+                return ties;
+            });
+            if (stage == PICK_DRAW) {
+                if (tid == 0) out[r] = (int)at.ord;
+                return;
+            }
+            if (stage == PICK_K || stage == PICK_P) {
+                ties_of = 0;
+                if (reached) {                                    // (else there are fewer: all stay)
+                    const uint32_t key = ~at.ord;
+                    set.cut = key == set.key ? set.cut : INT_MAX;
+                    set.key = key;
+                    // ties are alike in weight: where not all are needed it is those of the smallest indices that reach what is asked for
+                    if (at.need < at.above + at.inside) {
+                        ties_of = 1;
+                        tie_key = key;
+                        ties = at.need - at.above;
+                    }
+                }
+            } else {
+                set.cut = (int)at.ord;
+                ties_of = 0;
+            }
+            stage = ties_of ? stage + 1 : stage <= PICK_K_TIES && by_p ? PICK_P : PICK_DRAW;
+            if (stage == PICK_DRAW && from_row) break;
+        }
+    }
+    pick_from_row(sh, row, u, weights, out + r, [&](float x, int index) {
+        return place(x) < (float)PICK_BINS && set.has(key_of(x), index) && weights.octaves(x) >= floor_y;
+    });
 }
 
 extern "C" int imparo_pick_rows(const float* logits, const float* temperature, const float* uniform, const int32_t* top_k,
