@@ -281,6 +281,7 @@ extern "C" int imparo_sample_rows(const float* logits, const float* temperature,
 #define PICK_FEW 256               // tokens that are compared with one another instead
 #define PICK_EACH 4                // tokens of the list a thread has at most
 #define PICK_CUT 44
+#define PICK_STEPS 512
 
 typedef unsigned long long u64;
 
@@ -330,7 +331,7 @@ struct PickShared {
     u64 level[2][1 << PICK_BITS];     // used in turn: while one is read the other is cleared
     float list_x[PICK_EACH * 1024];
     int list_index[PICK_EACH * 1024];
-    double table[32];                 // 2^(i / 32)
+    double table[PICK_STEPS];         // 2^(i / PICK_STEPS)
     u64 waves[16], turns[132];
     float tops[16];
     u64 few_ord[PICK_FEW], few_weight[PICK_FEW], few_mass[2][PICK_FEW], few_sum[2];
@@ -341,26 +342,38 @@ struct PickShared {
     uint32_t key_low, key_high;
 };
 
-// Weights of a row: 2^y 2^44 to the nearest integer, y = (x - top) c1 <= 0, as an integer in a double. y 32 = n + f with n whole, 2^(n / 32)
-// out of a table and an exponent, and 2^(f / 32), |f| <= 1/2, from its power series, cut where the next term is below 2^-48; rounded by
-// an addition of 2^52, whose low bits then are the integer.
+// 2^(i / PICK_STEPS): e^z as its power series up to z^17 / 17!, z < 0.7, below a tenth of a float64's step
+struct PickTable {
+    double v[PICK_STEPS];
+    constexpr PickTable() : v() {
+        for (int i = 0; i < PICK_STEPS; ++i) {
+            const double z = 0.69314718055994530942 * i / PICK_STEPS;
+            double sum = 1.0;
+            for (int n = 17; n > 0; --n) sum = 1.0 + sum * z / n;
+            v[i] = sum;
+        }
+    }
+};
+static __device__ const PickTable pick_table = PickTable();
+
+// Weights of a row: 2^y 2^44 to the nearest integer, y = (x - top) c1 <= 0, for y above -45 (what is asked about lies in one of the bins).
+// y 512 = n + f with n whole, 2^(n / 512) out of a table and an exponent, and 2^(f / 512), |f| <= 1/2, from its power series, cut where the next term
+// is below 2^-46; rounded by an addition of 2^52, whose low bits then are the integer.
 struct PickWeights {
-    double top, c32;
+    static_assert(PICK_STEPS == 1 << 9, "the shift below");
+    double top, c;                    // c1 PICK_STEPS
     const double* table;
     __device__ __forceinline__ u64 operator()(float x) const {
-        constexpr double MAGIC = 6755399441055744.0, L = 0.69314718055994530942 / 32;
-        const double d = (double)x - top, t = fma(d, c32, MAGIC), f = fma(d, c32, -(t - MAGIC));
+        constexpr double MAGIC = 6755399441055744.0, L = 0.69314718055994530942 / PICK_STEPS;
+        const double d = (double)x - top, t = fma(d, c, MAGIC), f = fma(d, c, -(t - MAGIC));
         const int n = __double2loint(t);
-        double p = fma(f, L * L * L * L * L / 120, L * L * L * L / 24);
-        p = fma(f, p, L * L * L / 6);
-        p = fma(f, p, L * L / 2);
+        double p = fma(f, L * L * L / 6, L * L / 2);
         p = fma(f, p, L);
-        p = fma(f, p, 1.0);
-        const double v = ldexp(p * table[n & 31], (n >> 5) + PICK_CUT) + 4503599627370496.0;
-        const u64 whole = (u64)__double_as_longlong(v) & 0xFFFFFFFFFFFFFull;
-        return d * c32 >= -32.0 * PICK_CUT - 16.0 ? whole : 0;
+        p = fma(f, p, 1.0) * table[n & (PICK_STEPS - 1)];
+        const double v = __hiloint2double(__double2hiint(p) + (((n >> 9) + PICK_CUT) << 20), __double2loint(p)) + 4503599627370496.0;
+        return (u64)__double_as_longlong(v) & 0xFFFFFFFFFFFFFull;
     }
-    __device__ __forceinline__ double octaves(float x) const { return ((double)x - top) * c32 * 0.03125; }
+    __device__ __forceinline__ double octaves(float x) const { return ((double)x - top) * c * (1.0 / PICK_STEPS); }
 };
 
 // The bin of sh.hist where the running sum reaches what is asked for: `need`, or for share >= 0 that share of all. Leaves bin,
@@ -778,7 +791,7 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
     row.open(row_at, vocab);
     float own_top = -INFINITY;                                    // the largest of this thread's
     auto largest = [&](const float (&x)[4]) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); };
-    if (tid < 32) sh.table[tid] = exp2((double)tid * 0.03125);
+    for (int i = tid; i < PICK_STEPS; i += THREADS) sh.table[i] = pick_table.v[i];
     for (int b = tid; b < PICK_BINS; b += THREADS) sh.hist[b] = 0;
     for (int b = tid; b < 2 << PICK_BITS; b += THREADS) (&sh.level[0][0])[b] = 0;
     if (tid == 0) sh.n_list = 0;
@@ -792,18 +805,20 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
         sample_row(row_at, 0.f, u, out + r, vocab);
         return;
     }
-    const double c1 = 1.44269504088896340736 / (double)temp;
-    const PickWeights weights{(double)top, 32.0 * c1, sh.table};
+    // (the bins are float32: a temperature below 1.4e-36 counts as that, and tells logits apart that differ by 4e-35)
+    const double c1 = fmin(1.44269504088896340736 / (double)temp, 1.0e36);
+    const PickWeights weights{(double)top, c1 * PICK_STEPS, sh.table};
     const double floor_y = by_m ? fmax(-(double)PICK_CUT, log2((double)fminf(mp, 1.f))) : -(double)PICK_CUT;
     // bins an octave, and a unit of the logit: a logit d below the top is in bin d bin_scale
     constexpr float BINS_AN_OCTAVE = (float)PICK_BINS / PICK_CUT;
-    const float bin_scale = BINS_AN_OCTAVE * fminf((float)c1, 1.0e36f);
+    const float bin_scale = BINS_AN_OCTAVE * (float)c1;
     auto place = [&](float x) { return (top - x) * bin_scale; };
 
     // ---- how far down the list has to reach: `limit`, a number of bins
     float limit = (float)PICK_BINS;
     const double share = (double)fmaxf(p, 0.f);
     u64 need_p = 0;
+    bool too_many = false;                                        // (of no bearing on the result: with a list of the wrong kind the other way is taken)
     if (by_k) {
         if (k <= THREADS / 2) {
             // the k-th largest of the threads' maxima: so many logits at least are no smaller, and not many more
@@ -833,6 +848,18 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
         pick_bin(sh, 0, share);
         need_p = sh.need;
         limit = (float)(sh.bin + 1);
+        // about how many tokens that is, from what the bins hold and a token of a bin weighs
+        float about = 0.f;
+        for (int i = 0; i < PICK_BINS / THREADS; ++i) {
+            const int b = tid * (PICK_BINS / THREADS) + i;
+            if (b <= sh.bin) about += (float)sh.hist[b] * __builtin_amdgcn_exp2f(((float)b + 0.5f) / BINS_AN_OCTAVE - (float)PICK_CUT);
+        }
+        about = wave_sum(about);
+        if (lane == 0) sh.tops[wave] = about;
+        __syncthreads();
+        about = 0.f;
+        for (int w = 0; w < WAVES; ++w) about += sh.tops[w];
+        too_many = about > (float)ROOM;
     }
     // (a token that min-p takes out need not be listed, unless top-p asks for the sum of the k largest)
     if (by_m && !(by_k && by_p)) limit = fminf(limit, (float)(-floor_y * (double)BINS_AN_OCTAVE) * 1.0001f + 0.01f);
@@ -851,7 +878,8 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
                 }
         }
     };
-    row.each([&](const float (&x)[4], int index) { enlist(x, index, -1.f, limit); });
+    if (!too_many || by_m) row.each([&](const float (&x)[4], int index) { enlist(x, index, -1.f, limit); });
+    else if (tid == 0) sh.n_list = ROOM + 1;
     __syncthreads();
     PickSet set{0u, INT_MAX};
     const uint32_t key_high = key_of(top);
@@ -934,9 +962,18 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
             if (stage == PICK_DRAW && from_row) break;
         }
     }
-    pick_from_row(sh, row, u, weights, out + r, [&](float x, int index) {
-        return place(x) < (float)PICK_BINS && set.has(key_of(x), index) && weights.octaves(x) >= floor_y;
-    });
+    // what is kept, as a logit: all above `edge`, and so many as it. min-p's own border is the smallest logit that passes it
+    float edge = set.key ? float_of(set.key) : -INFINITY;
+    int cut = set.cut;
+    float lowest = fmaxf((float)((double)top + floor_y / c1), -3.0e38f);
+    auto next = [](float x, int up) { return float_of(key_of(x) + up); };
+    for (int i = 0; i < 8 && weights.octaves(next(lowest, -1)) >= floor_y; ++i) lowest = next(lowest, -1);
+    for (int i = 0; i < 16 && weights.octaves(lowest) < floor_y; ++i) lowest = next(lowest, 1);
+    if (lowest > edge) {
+        edge = lowest;
+        cut = INT_MAX;
+    }
+    pick_from_row(sh, row, u, weights, out + r, [&](float x, int index) { return x > edge || (x == edge && index <= cut); });
 }
 
 extern "C" int imparo_pick_rows(const float* logits, const float* temperature, const float* uniform, const int32_t* top_k,
