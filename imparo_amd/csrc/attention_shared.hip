@@ -436,7 +436,8 @@ extern "C" int imparo_attention_shared_parts(int n_rows, int heads, int kv_heads
 }
 
 extern "C" int imparo_attention_decode_shared(const void* q, const void* k_cache, const void* v_cache, void* out, float* part_o,
-                                              float* part_ml, const int32_t* rows, int n_rows, const int32_t* group_start, int n_groups,
+                                              float* part_ml, int64_t part_o_floats, int64_t part_ml_floats, const int32_t* rows, int n_rows,
+                                              const int32_t* group_start, int n_groups,
                                               const int32_t* shared, const int32_t* seg_start, const int32_t* positions,
                                               const int32_t* block_table, int table_stride, int page_size, int heads, int kv_heads,
                                               int head_dim, int n_pages, float scale, int window, int max_shared, int max_own,
@@ -450,7 +451,9 @@ extern "C" int imparo_attention_decode_shared(const void* q, const void* k_cache
         return IMPARO_BAD_ARGUMENT;
     if (n_rows == 0) return IMPARO_OK;
     const SharedShape s = shared_shape(n_rows, heads, kv_heads, n_groups, max_group, max_shared, max_own);
-    if (s.n_pre + s.n_own && (!part_o || !part_ml)) return IMPARO_BAD_ARGUMENT;
+    const long long parts = (long long)n_rows * heads * (s.n_pre + s.n_own);
+    if (parts && (!part_o || !part_ml)) return IMPARO_BAD_ARGUMENT;
+    if (part_o_floats < parts * head_dim || part_ml_floats < parts * 2) return IMPARO_SCRATCH_TOO_SMALL;
     const long long units = (long long)n_groups * kv_heads * s.n_pre;
     const long long pre_blocks = (units + 7) / 8 * 8 * s.pre_tiles, own_blocks = (long long)n_rows * kv_heads * s.own_tiles * s.n_own;
     if (pre_blocks + own_blocks > 1 << 30 || (long long)n_rows * heads > 1 << 30) return IMPARO_BAD_ARGUMENT;

@@ -67,9 +67,9 @@ _SIGNATURES = {
     "imparo_attention_decode_static": [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, F, I, I, P],
     "imparo_load_code": [],
     "imparo_attention_shared_parts": [I, I, I, I, I, I, I],
-    # q, k_cache, v_cache, out, part_o, part_ml, rows, n_rows, group_start, n_groups, shared, seg_start, positions, table, stride, page,
+    # q, k_cache, v_cache, out, part_o, part_ml, floats of each, rows, n_rows, group_start, n_groups, shared, seg_start, positions, table, stride, page,
     # heads, kv_heads, head_dim, n_pages, scale, window, max_shared, max_own, max_group, stream
-    "imparo_attention_decode_shared": [P, P, P, P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, F, I, I, I, I, P],
+    "imparo_attention_decode_shared": [P, P, P, P, P, P, c_int64, c_int64, P, I, P, I, P, P, P, P, I, I, I, I, I, I, F, I, I, I, I, P],
     "imparo_step_tables_max_rows": [],
     # lengths, new_tokens, leader, shared, pages, n_pages, page_size, n_rows, table, width, seg_start, positions, row_of_token, slots,
     # n_tokens, lists, counts, stream

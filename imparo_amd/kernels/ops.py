@@ -36,6 +36,10 @@ def _dev(t: Optional[torch.Tensor], what: str, dtype=None, shape=None) -> int:
     """Checks a tensor and returns its device address (0 for None)."""
     if t is None:
         return 0
+    # (one condition for the call that is right: the checks of a small launch cost the host more than the launch)
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous() and (dtype is None or t.dtype is dtype)
+            and (shape is None or t.shape == shape)):
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor):
         raise KernelArgumentError(f"{what} is not a tensor")
     if t.device.type != "cuda":
@@ -51,7 +55,7 @@ def _dev(t: Optional[torch.Tensor], what: str, dtype=None, shape=None) -> int:
 
 def _here(t: torch.Tensor, what: str) -> None:
     """Refuses a tensor of another GPU than the current one, whose stream the launch goes to."""
-    if t.device.type == "cuda" and t.device.index != torch.cuda.current_device():
+    if t.is_cuda and t.get_device() != torch.cuda.current_device():
         raise KernelArgumentError(f"{what} is on {t.device}, the current device is {torch.cuda.current_device()}")
 
 
@@ -78,14 +82,15 @@ class on_current_stream:
 def _stream() -> int:
     if _launch_stream is not None:
         return _launch_stream
-    return torch.cuda.current_stream().cuda_stream
+    # (the address alone: the library's object around it takes 2.6 us to make, half of what a launch takes)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _check(status: int, name: str) -> None:
     if status == 0:
         return
     why = {1: "an argument was refused (size or pointer the kernel cannot take)",
-           2: "the launch failed"}.get(status, f"status {status}")
+           2: "the launch failed", 3: "the scratch is too small"}.get(status, f"status {status}")
     raise KernelArgumentError(f"{name}: {why}")
 
 
@@ -239,6 +244,9 @@ def place_tokens(ids: torch.Tensor, dst: torch.Tensor, src: torch.Tensor, src_in
     return ids
 
 
+STEP_TABLES_MAX_ROWS = 4096       # rows that step_tables takes (imparo_step_tables_max_rows)
+
+
 def step_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, pages: torch.Tensor, page_size: int, block_table: torch.Tensor,
                 seg_start: torch.Tensor, positions: torch.Tensor, row_of_token: torch.Tensor, slots: Optional[torch.Tensor],
                 lists: torch.Tensor, counts: torch.Tensor, leader: Optional[torch.Tensor] = None,
@@ -256,8 +264,8 @@ def step_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, pages: torch.Te
         raise KernelArgumentError(f"step_tables: page size must be a power of two, got {page_size}")
     if (leader is None) != (shared is None):
         raise KernelArgumentError("step_tables: leaders and shared pages are given together")
-    if n > library().imparo_step_tables_max_rows():
-        raise KernelArgumentError(f"step_tables: {n} rows; at most {library().imparo_step_tables_max_rows()} are taken")
+    if n > STEP_TABLES_MAX_ROWS:
+        raise KernelArgumentError(f"step_tables: {n} rows; at most {STEP_TABLES_MAX_ROWS} are taken")
     if block_table.dim() != 2 or block_table.shape[1] < 1 or positions.dim() != 1 or pages.dim() != 1:
         raise KernelArgumentError("step_tables: a [rows, pages] block table and one position a token are needed")
     _here(lengths, "lengths")
@@ -624,16 +632,15 @@ def attention_decode_shared(q, k_cache, v_cache, out, part_o, part_ml, rows, n_r
     if seg_start.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] != seg_start.shape[0] or block_table.shape[1] < 1:
         raise KernelArgumentError(f"attention_decode_shared: a block table of {list(block_table.shape)} does not go with "
                                   f"{list(seg_start.shape)} rows")
-    parts = attention_shared_parts(n_rows, heads, kv_heads, head_dim, n_groups, max_group, max_shared, max_own)
-    if part_o.numel() < n_rows * heads * parts * head_dim or part_ml.numel() < n_rows * heads * parts * 2:
-        raise KernelArgumentError(f"attention_decode_shared: the scratch for {parts} parts is too small")
+    if min(max_shared, max_own, max_group) < 0 or max(max_shared, max_own) > 1 << 30:
+        raise KernelArgumentError("attention_decode_shared: a bound is negative, or above 2^30")
     _check(library().imparo_attention_decode_shared(
         _dev(q, "q"), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _dev(part_o, "partial outputs", torch.float32),
-        _dev(part_ml, "partial sums", torch.float32), _dev(rows, "decode rows", torch.int32), n_rows,
+        _dev(part_ml, "partial sums", torch.float32), part_o.numel(), part_ml.numel(), _dev(rows, "decode rows", torch.int32), n_rows,
         _dev(group_start, "group_start", torch.int32), n_groups, _dev(shared, "shared keys", torch.int32, (n_groups,)),
         _dev(seg_start, "seg_start", torch.int32), _dev(positions, "positions", torch.int32, (n,)),
         _dev(block_table, "block table", torch.int32), block_table.shape[1], page_size, heads, kv_heads, head_dim, n_pages,
-        float(scale), int(window or 0), int(max_shared), int(max_own), int(max_group), _stream()), "attention_decode_shared")
+        scale, window or 0, max_shared, max_own, max_group, _stream()), "attention_decode_shared")
     return out
 
 

@@ -63,7 +63,8 @@ def test_lengths_that_are_negative_or_long():
 
 
 def test_most_rows():
-    n = ops().library().imparo_step_tables_max_rows()
+    n = ops().STEP_TABLES_MAX_ROWS
+    assert n == ops().library().imparo_step_tables_max_rows()
     run([i % 40 for i in range(n)], [1] * n, list(range(3 * n)), 16, 3, n)
     with pytest.raises(ops().KernelArgumentError, match="at most"):
         run([1] * (n + 1), [1] * (n + 1), [], 16, 1, 1)
