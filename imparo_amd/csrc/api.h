@@ -347,7 +347,7 @@ int imparo_attention_decode(const void* q, const void* k_cache, const void* v_ca
 // softmax over each row's keys 0 .. position (under `window` the last so many of them; a position below 0 sees nothing and gives
 // zeros); weights are rounded to bfloat16 before they meet the values. part_o [n_rows, heads, parts, head_dim] and part_ml [n_rows,
 // heads, parts, 2] float32 hold the results of parts of the keys, with parts = imparo_attention_shared_parts(...); too few of them are IMPARO_SCRATCH_TOO_SMALL.
-int imparo_attention_shared_parts(int n_rows, int heads, int kv_heads, int head_dim, int n_groups, int max_group, int max_shared, int max_own);
+int imparo_attention_shared_parts(int n_rows, int heads, int kv_heads, int n_groups, int max_group, int max_shared, int max_own);
 int imparo_attention_decode_shared(const void* q, const void* k_cache, const void* v_cache, void* out, float* part_o,
                                    float* part_ml, int64_t part_o_floats, int64_t part_ml_floats, const int32_t* rows, int n_rows, const int32_t* group_start, int n_groups,
                                    const int32_t* shared, const int32_t* seg_start, const int32_t* positions,

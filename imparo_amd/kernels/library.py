@@ -66,7 +66,7 @@ _SIGNATURES = {
     "imparo_fill_sites": [P, P, P, I, I, P],
     "imparo_attention_decode_static": [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, F, I, I, P],
     "imparo_load_code": [],
-    "imparo_attention_shared_parts": [I, I, I, I, I, I, I, I],
+    "imparo_attention_shared_parts": [I, I, I, I, I, I, I],
     # q, k_cache, v_cache, out, part_o, part_ml, floats of each, rows, n_rows, group_start, n_groups, shared, seg_start, positions, table, stride, page,
     # heads, kv_heads, head_dim, n_pages, scale, window, max_shared, max_own, max_group, stream
     "imparo_attention_decode_shared": [P, P, P, P, P, P, c_int64, c_int64, P, I, P, I, P, P, P, P, I, I, I, I, I, I, F, I, I, I, I, P],

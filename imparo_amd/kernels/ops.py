@@ -605,8 +605,8 @@ def attention_shared_parts(n_rows: int, heads: int, kv_heads: int, head_dim: int
         raise KernelArgumentError(f"attention_shared_parts: {heads} heads of {head_dim} by {kv_heads} are not taken")
     if min(n_rows, n_groups, max_group, max_shared, max_own) < 0 or max(max_shared, max_own) > 1 << 30:
         raise KernelArgumentError("attention_shared_parts: a bound is negative, or above 2^30")
-    return int(library().imparo_attention_shared_parts(int(n_rows), int(heads), int(kv_heads), int(head_dim), int(n_groups),
-                                                       int(max_group), int(max_shared), int(max_own)))
+    return int(library().imparo_attention_shared_parts(int(n_rows), int(heads), int(kv_heads), int(n_groups), int(max_group),
+                                                       int(max_shared), int(max_own)))
 
 
 def attention_decode_shared(q, k_cache, v_cache, out, part_o, part_ml, rows, n_rows: int, group_start, shared, seg_start, positions,
