@@ -23,11 +23,13 @@
 
 #define SHARED_WAVES 4
 #define SHARED_KEYS 64             // shared keys of a tile
-#define SHARED_MIN_SPLIT 256       // and of a part at least
-#define SHARED_BLOCKS 512          // blocks that shared keys are cut for, two a CU
+#define SHARED_MIN_SPLIT 256       // and of a part at least, of so many keys that these make many parts
+#define SHARED_FEW_SPLIT 128       // and else (448 keys in parts of 128 | 256: 10.7 | 11.7 us; 4,096: 19.9 | 18.3, with twice the parts to add up)
+#define SHARED_SPLIT 1024          // and of a part where there is a block a CU
+#define SHARED_BLOCKS 512          // blocks that shared keys are cut for at most, two a CU
 #define OWN_KEYS 32                // a row's own keys of a tile
 #define OWN_MIN_SPLIT 64           // and of a part at least
-#define OWN_WAVES 4096             // waves that own keys are cut for
+#define OWN_WAVES 3072             // waves that own keys are cut for
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -38,6 +40,8 @@ union SharedFrag {
     bf16x8 v;
 };
 __device__ __forceinline__ u32x4 load16(const bf16_t* p) { return *reinterpret_cast<const u32x4*>(p); }
+// the same of lines that are read once and whole by one instruction: they need not stay in a cache
+__device__ __forceinline__ u32x4 load16_once(const bf16_t* p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)); }
 // a piece of values at keys key .. key + 7 with those outside [lo, hi] zeroed, whatever stands there
 __device__ __forceinline__ u32x4 only_between(u32x4 v, int key, int lo, int hi) {
 #pragma unroll
@@ -376,7 +380,7 @@ struct OwnWave {
                 const size_t first = (a_page(a, __builtin_amdgcn_readfirstlane(page[0])) * a.kv_heads + kvh) << a.page_shift;
                 const bf16_t *k = a.k + (first + (key0 & mask)) * D, *v = a.v + first * D + (key0 & mask);
 #pragma unroll
-                for (int j = 0; j < ND; ++j) kr[j] = load16(k + 8 * (lane + j * WAVE));
+                for (int j = 0; j < ND; ++j) kr[j] = load16_once(k + 8 * (lane + j * WAVE));
 #pragma unroll
                 for (int j = 0; j < ND; ++j) vr[j] = load16(v + (((lane + j * WAVE) / 4 << a.page_shift) + 8 * (lane & 3)));
             } else {
@@ -558,15 +562,20 @@ static SharedShape shared_shape(int n_rows, int heads, int kv_heads, int n_group
     s.query_waves = queries > 64 ? 4 : 2;
     s.pre_tiles = max_shared > 0 && n_groups > 0 ? (int)((queries + 32 * s.query_waves - 1) / (32 * s.query_waves)) : 0;
     s.own_tiles = (per + 15) / 16;
-    auto cut = [](long long wanted, long long units, int keys, int least, int step, int& n, int& split) {
-        n = clamped(wanted / units, 1, (keys + least - 1) / least);
+    auto cut = [](long long pieces, int keys, int least, int step, int& n, int& split) {
+        n = clamped(pieces, 1, (keys + least - 1) / least);
         split = ((keys + n - 1) / n + step - 1) / step * step;
         n = (keys + split - 1) / split;
     };
     s.n_pre = s.n_own = 0, s.pre_split = SHARED_KEYS, s.own_split = OWN_KEYS;
-    if (s.pre_tiles) cut(SHARED_BLOCKS, (long long)n_groups * kv_heads * s.pre_tiles, max_shared, SHARED_MIN_SPLIT, SHARED_KEYS, s.n_pre, s.pre_split);
-    // (own keys are counted from a multiple of a tile, up to a tile less one below the first)
-    if (max_own > 0) cut(OWN_WAVES, (long long)n_rows * kv_heads * s.own_tiles, max_own + OWN_KEYS - 1, OWN_MIN_SPLIT, OWN_KEYS, s.n_own, s.own_split);
+    if (s.pre_tiles) {
+        // a part costs its results' way to memory and back: from a block a CU on parts are long ones (4,096 keys of 1,024 queries a kv head in parts of
+        // 512, 1,024: 151, 134 us beside the own keys; 32,768 keys of 256 queries in parts of 1,024, 2,048: 48, 54)
+        const long long units = (long long)n_groups * kv_heads * s.pre_tiles, few = SHARED_BLOCKS / 2 / units, most = SHARED_BLOCKS / units;
+        cut(clamped(max_shared / SHARED_SPLIT, few, most), max_shared, max_shared > 8 * SHARED_MIN_SPLIT ? SHARED_MIN_SPLIT : SHARED_FEW_SPLIT, SHARED_KEYS, s.n_pre, s.pre_split);
+    }
+    // (own keys are counted from a multiple of OWN_KEYS, up to one less below the first)
+    if (max_own > 0) cut(OWN_WAVES / ((long long)n_rows * kv_heads * s.own_tiles), max_own + OWN_KEYS - 1, OWN_MIN_SPLIT, OWN_KEYS, s.n_own, s.own_split);
     return s;
 }
 static bool shared_sizes_bad(int n_rows, int heads, int kv_heads, int n_groups, int max_group, int max_shared, int max_own) {
