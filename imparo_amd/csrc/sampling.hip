@@ -13,7 +13,7 @@ __device__ __forceinline__ Best better(Best a, Best b) {
     return (b.v > a.v || (b.v == a.v && b.i < a.i)) ? b : a;
 }
 
-__device__ __forceinline__ Best block_best(Best b, Best* scratch) {
+__device__ __forceinline__ Best block_best(Best b, Best* scratch, int threads) {
     b = better(b, Best{lane_xor<32>(b.v), lane_xor<32>(b.i)});
     b = better(b, Best{lane_xor<16>(b.v), lane_xor<16>(b.i)});
     b = better(b, Best{lane_xor<8>(b.v), lane_xor<8>(b.i)});
@@ -21,7 +21,7 @@ __device__ __forceinline__ Best block_best(Best b, Best* scratch) {
     b = better(b, Best{lane_xor<2>(b.v), lane_xor<2>(b.i)});
     b = better(b, Best{lane_xor<1>(b.v), lane_xor<1>(b.i)});
     const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-    const int n_waves = (blockDim.x + WAVE - 1) / WAVE;
+    const int n_waves = (threads + WAVE - 1) / WAVE;
     __syncthreads();
     if (lane == 0) scratch[wave] = b;
     __syncthreads();
@@ -30,7 +30,7 @@ __device__ __forceinline__ Best block_best(Best b, Best* scratch) {
     return r;
 }
 
-__device__ __forceinline__ Best row_best(const float* __restrict__ row, int vocab, Best* scratch) {
+__device__ __forceinline__ Best row_best(const float* __restrict__ row, int vocab, Best* scratch, int threads) {
     Best b;
     b.v = -INFINITY;
     b.i = INT_MAX;
@@ -41,7 +41,7 @@ __device__ __forceinline__ Best row_best(const float* __restrict__ row, int voca
         // and a choice of index for every value were a third of the time (one row of 65,536 9.0 us, so 6.2).
         const float4* row4 = reinterpret_cast<const float4*>(row);
         const int n4 = vocab >> 2;
-        if (n4 <= (int)blockDim.x) {
+        if (n4 <= threads) {
             // one load a thread: the maximum and its index together, one meeting of the block (a row of 1,000 in two 3.8 us)
             const float4 v = row4[min((int)threadIdx.x, n4 - 1)];
             const float vs[4] = {v.x, v.y, v.z, v.w};
@@ -51,17 +51,17 @@ __device__ __forceinline__ Best row_best(const float* __restrict__ row, int voca
                     b.v = vs[j];
                     b.i = 4 * (int)threadIdx.x + j;
                 }
-            b = block_best(b, scratch);
+            b = block_best(b, scratch, threads);
             if (b.i == INT_MAX) b.i = 0;   // every value was NaN
             return b;
         }
         constexpr int DEEP = 16;
         float m = -INFINITY;
         int met = 0;
-        for (int first = threadIdx.x; first < n4; first += DEEP * (int)blockDim.x) {
+        for (int first = threadIdx.x; first < n4; first += DEEP * threads) {
             float4 v[DEEP];
 #pragma unroll
-            for (int k = 0; k < DEEP; ++k) v[k] = row4[min(first + k * (int)blockDim.x, n4 - 1)];
+            for (int k = 0; k < DEEP; ++k) v[k] = row4[min(first + k * threads, n4 - 1)];
             float mm = -INFINITY;
 #pragma unroll
             for (int k = 0; k < DEEP; ++k) mm = fmaxf(mm, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
@@ -71,7 +71,7 @@ __device__ __forceinline__ Best row_best(const float* __restrict__ row, int voca
             }
         }
         float top = wave_max(m);
-        const int n_waves = (blockDim.x + WAVE - 1) / WAVE;
+        const int n_waves = (threads + WAVE - 1) / WAVE;
         if ((threadIdx.x & (WAVE - 1)) == 0) scratch[threadIdx.x / WAVE].v = top;
         __syncthreads();
         float tops[16];
@@ -83,10 +83,10 @@ __device__ __forceinline__ Best row_best(const float* __restrict__ row, int voca
             if (m == top) {
                 float4 v[DEEP];
 #pragma unroll
-                for (int k = 0; k < DEEP; ++k) v[k] = row4[min(met + k * (int)blockDim.x, n4 - 1)];
+                for (int k = 0; k < DEEP; ++k) v[k] = row4[min(met + k * threads, n4 - 1)];
 #pragma unroll
                 for (int k = DEEP - 1; k >= 0; --k) {
-                    const int i = min(met + k * (int)blockDim.x, n4 - 1);
+                    const int i = min(met + k * threads, n4 - 1);
                     const float vs[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
                     for (int j = 3; j >= 0; --j)
@@ -94,24 +94,24 @@ __device__ __forceinline__ Best row_best(const float* __restrict__ row, int voca
                 }
                 b.v = top;
             }
-            return block_best(b, scratch);
+            return block_best(b, scratch, threads);
         }
     }
-    for (int i = threadIdx.x; i < vocab; i += blockDim.x) {
+    for (int i = threadIdx.x; i < vocab; i += threads) {
         const float v = row[i];
         if (v > b.v || (v == b.v && i < b.i)) {
             b.v = v;
             b.i = i;
         }
     }
-    b = block_best(b, scratch);
+    b = block_best(b, scratch, threads);
     if (b.i == INT_MAX) b.i = 0;   // every value was NaN
     return b;
 }
 
 __global__ void k_argmax_rows(const float* __restrict__ logits, int32_t* __restrict__ out, int vocab) {
     __shared__ Best scratch[16];
-    const Best b = row_best(logits + (size_t)blockIdx.x * vocab, vocab, scratch);
+    const Best b = row_best(logits + (size_t)blockIdx.x * vocab, vocab, scratch, blockDim.x);
     if (threadIdx.x == 0) out[blockIdx.x] = b.i;
 }
 
@@ -132,18 +132,18 @@ extern "C" int imparo_argmax_rows(const float* logits, int32_t* out, int n_rows,
 // rows of 65,536 logits: 153 us with both chains reading LDS and memory value by value, 38 us so (28 us for rows of 16,384).
 #define SAMPLE_THREADS 1024
 __device__ __forceinline__ void sample_row(const float* __restrict__ row, float temp, float uniform, int32_t* __restrict__ out,
-                                           int vocab) {
+                                           int vocab, int threads) {
     __shared__ Best scratch[16];
     __shared__ __attribute__((aligned(16))) float sums[SAMPLE_THREADS], before[SAMPLE_THREADS];
     __shared__ int first_past, last_positive, found;
     __shared__ float cum_shared, target_shared;
-    const Best top = row_best(row, vocab, scratch);
+    const Best top = row_best(row, vocab, scratch, threads);
     if (!(temp > 0.f)) {
         if (threadIdx.x == 0) *out = top.i;
         return;
     }
     const float inv_t = 1.0f / temp;
-    const int tid = threadIdx.x, threads = blockDim.x;         // (a multiple of 16)
+    const int tid = threadIdx.x;                               // (threads: a multiple of 16)
     const int piece = (vocab + threads - 1) / threads;
     const int begin = min(vocab, tid * piece), end = min(vocab, begin + piece);
     float local = 0.f;
@@ -246,14 +246,17 @@ __device__ __forceinline__ void sample_row(const float* __restrict__ row, float 
 __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_rows(
     const float* __restrict__ logits, const float* __restrict__ temperature, const float* __restrict__ uniform,
     int32_t* __restrict__ out, int vocab) {
-    sample_row(logits + (size_t)blockIdx.x * vocab, temperature[blockIdx.x], uniform[blockIdx.x], out + blockIdx.x, vocab);
+    sample_row(logits + (size_t)blockIdx.x * vocab, temperature[blockIdx.x], uniform[blockIdx.x], out + blockIdx.x, vocab, blockDim.x);
 }
+
+// (the order of a row's sums depends on it)
+__host__ __device__ static inline int sample_threads(int vocab) { return vocab >= 16384 ? SAMPLE_THREADS : 256; }
 
 extern "C" int imparo_sample_rows(const float* logits, const float* temperature, const float* uniform, int32_t* out,
                                   int n_rows, int vocab, imparo_stream stream) {
     if (!logits || !temperature || !uniform || !out || n_rows < 0 || vocab <= 0) return IMPARO_BAD_ARGUMENT;
     if (n_rows == 0) return IMPARO_OK;
-    const int threads = vocab >= 16384 ? SAMPLE_THREADS : 256;
+    const int threads = sample_threads(vocab);
     k_sample_rows<<<n_rows, threads, 0, (hipStream_t)stream>>>(logits, temperature, uniform, out, vocab);
     return launch_status();
 }
@@ -269,13 +272,14 @@ extern "C" int imparo_sample_rows(const float* logits, const float* temperature,
 // fill 63 bits. A token below 2^-44 of the likeliest is not drawn: all of those together weigh less than 2^-25, under one
 // step of a 24-bit u.
 // One block a row, and what an instruction a logit costs is what the kernel costs (65,536 logits, 64 lanes a clock: 0.43 us each),
-// so the row is read few times (out of L2 after the first) and little is done a logit. First the largest; then a bound under
-// which nothing is kept, as a number of bins, 2,048 over the 44 octaves that weigh anything: for min-p its own; for top-k the k-th
-// largest of the threads' own maxima, as k logits at least are no smaller; for top-p alone the bin of a histogram of weights where p of them
-// is reached. The tokens above that go into a list, four a thread at most, and border, ties and pick are found in the list alone,
-// by histograms over eight bits of keys or indices at a time, one barrier each (list_find). A row whose kept tokens do not fit the list
-// lists the tokens of the border's bin only and picks in two further passes; if not even those fit, everything is done over
-// the row itself, pass by pass (pick_narrow).
+// so the row is read few times (out of L2 after the first) and little is done a logit. First the largest; then how far down anything is
+// kept, as a number of bins, 2,048 over the 44 octaves that weigh anything: for min-p its own; for top-k the k-th largest of the threads'
+// own maxima, as k logits at least are no smaller; for top-p alone the bin of a histogram of weights where p of them is reached. The tokens above
+// that go into a list, four a thread at most, and border, ties and pick are found in the list alone, every
+// token compared with every other where they are few, else by histograms over nine bits of keys or indices at a time (list_find). A row
+// that keeps more under top-p lists the tokens of the border's bin only, sums up the ones above by the runs they are in, and picks in the
+// run that u falls in. What fits neither (large top-k, thousands of ties) is done over the row itself, pass by pass (pick_narrow).
+#define PICK_THREADS 1024          // of short rows too: 5 of 1,003 under top-k with 256 threads 13.1 us, so 9.9; 8 of 16,000 under top-p 53 and 24
 #define PICK_BINS 2048
 #define PICK_BITS 9                // bits of a key or an index that a search in the list settles at a time
 #define PICK_FEW 256               // tokens that are compared with one another instead
@@ -329,8 +333,8 @@ __device__ __forceinline__ T wave_scan(T v) {                     // the sum ove
 struct PickShared {
     u64 hist[PICK_BINS];
     u64 level[2][1 << PICK_BITS];     // used in turn: while one is read the other is cleared
-    float list_x[PICK_EACH * 1024];
-    int list_index[PICK_EACH * 1024];
+    float list_x[PICK_EACH * PICK_THREADS];
+    int list_index[PICK_EACH * PICK_THREADS];
     double table[PICK_STEPS];         // 2^(i / PICK_STEPS)
     u64 waves[16], turns[132];
     float tops[16];
@@ -718,21 +722,11 @@ __device__ __forceinline__ void pick_narrow(PickShared& sh, const PickRow& row, 
     set.cut = sh.cut;
 }
 
-// The pick out of the row, for what `kept` says of a logit and its index: sums over the waves' runs, then all waves take the turns of the run
-// where u falls, then a wave the turn.
+// The pick out of the row, for what `kept` says of a logit and its index, where the sums over the waves' runs stand in sh.waves: all waves take the turns of
+// the run where u falls, then a wave the turn.
 template <typename K>
-__device__ __forceinline__ void pick_from_row(PickShared& sh, PickRow row, float u, const PickWeights& weights, int32_t* out, K kept) {
+__device__ __forceinline__ void pick_in_runs(PickShared& sh, PickRow row, float u, const PickWeights& weights, int32_t* out, K kept) {
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE, waves = blockDim.x / WAVE;
-    u64 mine = 0;
-    row.each([&](const float (&x)[4], int index) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (kept(x[j], index + j)) mine += weights(x[j]);
-    });
-    const u64 of_wave = wave_sum_u64(mine);
-    __syncthreads();
-    if (lane == 0) sh.waves[wave] = of_wave;
-    __syncthreads();
     u64 total = 0;
     for (int w = 0; w < waves; ++w) total += sh.waves[w];
     const u64 target = passed_at(u, total) - 1;
@@ -769,22 +763,36 @@ __device__ __forceinline__ void pick_from_row(PickShared& sh, PickRow row, float
         *out = row.first + c * 4 * WAVE + j;
     }
 }
+// The same, the sums first
+template <typename K>
+__device__ __forceinline__ void pick_from_row(PickShared& sh, const PickRow& row, float u, const PickWeights& weights, int32_t* out, K kept) {
+    u64 mine = 0;
+    row.each([&](const float (&x)[4], int index) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (kept(x[j], index + j)) mine += weights(x[j]);
+    });
+    mine = wave_sum_u64(mine);
+    __syncthreads();
+    if ((threadIdx.x & (WAVE - 1)) == 0) sh.waves[threadIdx.x / WAVE] = mine;
+    __syncthreads();
+    pick_in_runs(sh, row, u, weights, out, kept);
+}
 
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void k_pick_rows(
+__global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
     const float* __restrict__ logits, const float* __restrict__ temperature, const float* __restrict__ uniform,
     const int32_t* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p,
     int32_t* __restrict__ out, int vocab) {
     __shared__ PickShared sh;
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
-    constexpr int WAVES = THREADS / WAVE, ROOM = PICK_EACH * THREADS;
+    constexpr int THREADS = PICK_THREADS, WAVES = THREADS / WAVE, ROOM = PICK_EACH * THREADS;
     const float* row_at = logits + (size_t)r * vocab;
     const float temp = temperature[r], u = uniform[r];
     const int k = top_k ? top_k[r] : 0;
     const float p = top_p ? top_p[r] : 1.f, mp = min_p ? min_p[r] : 0.f;
     const bool by_k = k > 0 && k < vocab, by_p = p < 1.f, by_m = mp > 0.f;
     if (!(temp > 0.f) || !(by_k || by_p || by_m)) {               // greedy, or the whole distribution
-        sample_row(row_at, temp, u, out + r, vocab);
+        if (tid < sample_threads(vocab)) sample_row(row_at, temp, u, out + r, vocab, sample_threads(vocab));   // (in whole waves; the others are done)
         return;
     }
     PickRow row;
@@ -802,7 +810,7 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sh.tops[w]);
     if (!(top < INFINITY) || !(top > -INFINITY)) {                // an infinite logit takes it, or there is none to take
-        sample_row(row_at, 0.f, u, out + r, vocab);
+        if (tid < sample_threads(vocab)) sample_row(row_at, 0.f, u, out + r, vocab, sample_threads(vocab));
         return;
     }
     // (the bins are float32: a temperature below 1.4e-36 counts as that, and tells logits apart that differ by 4e-35)
@@ -818,7 +826,7 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
     float limit = (float)PICK_BINS;
     const double share = (double)fmaxf(p, 0.f);
     u64 need_p = 0;
-    bool too_many = false;                                        // (of no bearing on the result: with a list of the wrong kind the other way is taken)
+    bool window = false;                                          // the list has the tokens of the border's bin only: not all that is kept is in it
     if (by_k) {
         if (k <= THREADS / 2) {
             // the k-th largest of the threads' maxima: so many logits at least are no smaller, and not many more
@@ -859,61 +867,71 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
         __syncthreads();
         about = 0.f;
         for (int w = 0; w < WAVES; ++w) about += sh.tops[w];
-        too_many = about > (float)ROOM;
+        window = about > (float)ROOM && !by_m;                    // (of no bearing on the result: with too many for the list it is the other way after all)
     }
+    const float border = (float)sh.bin;
     // (a token that min-p takes out need not be listed, unless top-p asks for the sum of the k largest)
     if (by_m && !(by_k && by_p)) limit = fminf(limit, (float)(-floor_y * (double)BINS_AN_OCTAVE) * 1.0001f + 0.01f);
 
     // ---- the list
-    auto enlist = [&](const float (&x)[4], int index, float from, float to) {
-        if (place(largest(x)) < to) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (place(x[j]) < to && place(x[j]) >= from) {
-                    const int at = atomicAdd(&sh.n_list, 1);
-                    if (at < ROOM) {
-                        sh.list_x[at] = x[j];
-                        sh.list_index[at] = index + j;
-                    }
-                }
+    auto enlist = [&](float x, int index) {
+        const int at = atomicAdd(&sh.n_list, 1);
+        if (at < ROOM) {
+            sh.list_x[at] = x;
+            sh.list_index[at] = index;
         }
     };
-    if (!too_many || by_m) row.each([&](const float (&x)[4], int index) { enlist(x, index, -1.f, limit); });
-    else if (tid == 0) sh.n_list = ROOM + 1;
-    __syncthreads();
+    if (!window) {
+        row.each([&](const float (&x)[4], int index) {
+            if (place(largest(x)) < limit) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (place(x[j]) < limit) enlist(x[j], index + j);
+            }
+        });
+        __syncthreads();
+        if (by_p && !by_k && sh.n_list > ROOM) {
+            window = true;
+            __syncthreads();
+            if (tid == 0) sh.n_list = 0;
+            __syncthreads();
+        }
+    }
+    if (window) {
+        limit = border + 1.f;
+        u64 sure = 0;                                             // what this wave's tokens above the border's bin weigh
+        row.each([&](const float (&x)[4], int index) {
+            if (place(largest(x)) < limit) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float at = place(x[j]);
+                    if (at < border) sure += weights(x[j]);
+                    else if (at < limit) enlist(x[j], index + j);
+                }
+            }
+        });
+        sure = wave_sum_u64(sure);
+        if (lane == 0) sh.turns[wave] = sure;
+        __syncthreads();
+        need_p -= sh.above;
+    }
     PickSet set{0u, INT_MAX};
-    const uint32_t key_high = key_of(top);
-    auto key_under = [&](float bins) { return key_of(top - bins / bin_scale * 1.0001f - fabsf(top) * 1.0e-5f); };   // (no lower place's key is above)
-    if (sh.n_list <= PICK_FEW) {
+    // (no listed token's key lies outside these)
+    const uint32_t key_high = window ? key_of(fminf(top, top - border / bin_scale * 0.9999f + fabsf(top) * 1.0e-5f)) : key_of(top);
+    const uint32_t key_low = key_of(top - limit / bin_scale * 1.0001f - fabsf(top) * 1.0e-5f);
+    if (!window && sh.n_list <= PICK_FEW) {
         pick_few<THREADS>(sh, weights, k, share, by_k, by_p, need_p, floor_y, u, out + r);
         return;
     }
     PickList list;
     list.turn = 0;
-    uint32_t key_low = key_under(limit);
     int stage = by_k ? PICK_K : by_p ? PICK_P : PICK_DRAW;
-    bool from_row = sh.n_list > ROOM;                             // too many for the list: the pick is made out of the row
-    if (from_row) {
-        bool border = false;
-        if (by_p && !by_k) {                                      // the tokens of the border's bin, and what is asked for beyond what lies above
-            const float bin = (float)sh.bin;
-            need_p -= sh.above;
-            __syncthreads();
-            if (tid == 0) sh.n_list = 0;
-            __syncthreads();
-            row.each([&](const float (&x)[4], int index) { enlist(x, index, bin, bin + 1.f); });
-            __syncthreads();
-            border = sh.n_list <= ROOM;
-            key_low = key_under(bin + 1.f);
-            if (!border) need_p += sh.above;
-        }
-        if (!border) {                                            // over the row itself
-            if (by_k) pick_narrow<true>(sh, row, set, top, bin_scale, weights, (u64)k, -1.0);
-            if (by_p) pick_narrow<false>(sh, row, set, top, bin_scale, weights, 0, share);
-            stage = PICK_DRAW;
-        }
-    }
-    if (!from_row || stage != PICK_DRAW) {
+    bool from_row = window || sh.n_list > ROOM;                   // the pick is made out of the row
+    bool listed = sh.n_list <= ROOM;
+    if (!listed) {                                                // too many for the list as well: over the row itself
+        if (by_k) pick_narrow<true>(sh, row, set, top, bin_scale, weights, (u64)k, -1.0);
+        if (by_p) pick_narrow<false>(sh, row, set, top, bin_scale, weights, 0, share);
+    } else {
         list.take(sh, weights, THREADS);
         Found at;
         int ties_of = 0;                                          // (the search behind the ties)
@@ -972,8 +990,21 @@ __global__ __launch_bounds__(THREADS) void k_pick_rows(
     if (lowest > edge) {
         edge = lowest;
         cut = INT_MAX;
+        listed = false;                                           // (the sums above the window hold what min-p takes out)
     }
-    pick_from_row(sh, row, u, weights, out + r, [&](float x, int index) { return x > edge || (x == edge && index <= cut); });
+    auto kept = [&](float x, int index) { return x > edge || (x == edge && index <= cut); };
+    if (window && listed) {                                       // the runs' sums: what lies above the window, and what is kept of it
+        if (tid < WAVES) sh.waves[tid] = sh.turns[tid];
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < PICK_EACH; ++e)
+            if (e < list.n && kept(list.x[e], list.index[e]))
+                atomicAdd(&sh.waves[(list.index[e] + row.skew) / (row.turns * 4 * WAVE)], list.weight[e]);
+        __syncthreads();
+        pick_in_runs(sh, row, u, weights, out + r, kept);
+    } else {
+        pick_from_row(sh, row, u, weights, out + r, kept);
+    }
 }
 
 extern "C" int imparo_pick_rows(const float* logits, const float* temperature, const float* uniform, const int32_t* top_k,
@@ -983,9 +1014,7 @@ extern "C" int imparo_pick_rows(const float* logits, const float* temperature, c
     if (n_rows == 0) return IMPARO_OK;
     if (!logits || !temperature || !uniform || !out || ((uintptr_t)logits & 3)) return IMPARO_BAD_ARGUMENT;
     hipStream_t s = (hipStream_t)stream;
-    // (a row without a filter goes through sample_row, whose sums depend on the threads: as many as imparo_sample_rows has)
-    if (vocab >= 16384) k_pick_rows<1024><<<n_rows, 1024, 0, s>>>(logits, temperature, uniform, top_k, top_p, min_p, out, vocab);
-    else k_pick_rows<256><<<n_rows, 256, 0, s>>>(logits, temperature, uniform, top_k, top_p, min_p, out, vocab);
+    k_pick_rows<<<n_rows, PICK_THREADS, 0, s>>>(logits, temperature, uniform, top_k, top_p, min_p, out, vocab);
     return launch_status();
 }
 
