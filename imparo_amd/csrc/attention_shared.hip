@@ -243,30 +243,37 @@ struct SharedBlock {
             ask_pages(key0 + 2 * SHARED_KEYS);
             __syncthreads();
             for (; key0 <= hi_all; key0 += SHARED_KEYS, buf ^= 1) {
+                // this wave's keys of the tile: all 64, or its half of them
+                constexpr int N = SHARED_KEYS / 32 / KW;
+                const int at = KW > 1 ? 32 * kw : 0, key = key0 + at;
+                if (__any(key <= hi && key + 32 * N - 1 >= lo)) {
+                    f32x16 s[N];
 #pragma unroll
-                for (int half = 0; half < SHARED_KEYS / 32 / KW; ++half) {
-                    const int at = 32 * (half + (KW > 1 ? kw : 0)), key = key0 + at;
-                    if (!__any(key <= hi && key + 31 >= lo)) continue;
-                    const bf16_t* krow = ks + buf * K_SIZE + (at + ((c & 16) | (c & 4) << 1 | (c & 8) >> 1 | (c & 3))) * LDK + 8 * h;
-                    f32x16 s;
+                    for (int n = 0; n < N; ++n) {
+                        const bf16_t* krow = ks + buf * K_SIZE + (at + 32 * n + ((c & 16) | (c & 4) << 1 | (c & 8) >> 1 | (c & 3))) * LDK + 8 * h;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+                        for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
 #pragma unroll
-                    for (int k = 0; k < ND; ++k) {
-                        SharedFrag f;
-                        f.u = load16(krow + 16 * k);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v, q[k].v, s, 0, 0, 0);
-                    }
-                    if (__any(valid && (key < lo || key + 31 > hi))) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int one = key + 16 * (r >> 3) + 8 * h + (r & 7);
-                            s[r] = one >= lo && one <= hi ? s[r] : -INFINITY;
+                        for (int k = 0; k < ND; ++k) {
+                            SharedFrag f;
+                            f.u = load16(krow + 16 * k);
+                            s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v, q[k].v, s[n], 0, 0, 0);
                         }
                     }
-                    float mx = fmaxf(s[0], s[1]);
+                    if (__any(valid && (key < lo || key + 32 * N - 1 > hi))) {
 #pragma unroll
-                    for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
+                        for (int n = 0; n < N; ++n)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const int one = key + 32 * n + 16 * (r >> 3) + 8 * h + (r & 7);
+                                s[n][r] = one >= lo && one <= hi ? s[n][r] : -INFINITY;
+                            }
+                    }
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int r = 0; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[n][r]), s[n][r + 1]);
                     float corr;
                     if (moved_reference(m, mx * a.scale, corr, [](float v) { return fmaxf(v, lane_xor<32>(v)); })) {
                         l *= corr;
@@ -276,26 +283,29 @@ struct SharedBlock {
                             for (int r = 0; r < 16; ++r) o[dt][r] *= corr;
                     }
                     const float from = m == -INFINITY ? 0.f : m;
-                    float sum = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale, -from));
-                        sum += s[r];
-                    }
-                    l += sum;
-                    SharedFrag p[2];
+                    for (int n = 0; n < N; ++n) {
+                        float sum = 0.f;
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        p[u].u = u32x4{f32x2_to_bf16x2(s[8 * u], s[8 * u + 1]), f32x2_to_bf16x2(s[8 * u + 2], s[8 * u + 3]),
-                                       f32x2_to_bf16x2(s[8 * u + 4], s[8 * u + 5]), f32x2_to_bf16x2(s[8 * u + 6], s[8 * u + 7])};
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            SharedFrag f;                         // (rows past the head: whatever stands there, never written out)
-                            f.u = load16(vs + buf * V_SIZE + (32 * dt + c) * LDV + at + 16 * u + 8 * h);
-                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v, p[u].v, o[dt], 0, 0, 0);
+                        for (int r = 0; r < 16; ++r) {
+                            s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.scale, -from));
+                            sum += s[n][r];
                         }
+                        l += sum;
+                        SharedFrag p[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            p[u].u = u32x4{f32x2_to_bf16x2(s[n][8 * u], s[n][8 * u + 1]), f32x2_to_bf16x2(s[n][8 * u + 2], s[n][8 * u + 3]),
+                                           f32x2_to_bf16x2(s[n][8 * u + 4], s[n][8 * u + 5]), f32x2_to_bf16x2(s[n][8 * u + 6], s[n][8 * u + 7])};
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                SharedFrag f;                     // (rows past the head: whatever stands there, never written out)
+                                f.u = load16(vs + buf * V_SIZE + (32 * dt + c) * LDV + at + 32 * n + 16 * u + 8 * h);
+                                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v, p[u].v, o[dt], 0, 0, 0);
+                            }
+                    }
                 }
                 if (key0 + SHARED_KEYS <= hi_all) {
                     keep_tile(key0 + SHARED_KEYS, buf ^ 1);

@@ -612,14 +612,15 @@ def attention_shared_parts(n_rows: int, heads: int, kv_heads: int, head_dim: int
 def attention_decode_shared(q, k_cache, v_cache, out, part_o, part_ml, rows, n_rows: int, group_start, shared, seg_start, positions,
                             block_table, scale: float, window: Optional[int], max_shared: int, max_own: int,
                             max_group: int) -> torch.Tensor:
-    """`attention_decode` for rows in groups that share a prefix: group g is the listed rows group_start[g] .. group_start[g + 1] - 1,
-    whose tables name the same pages for the keys 0 .. shared[g] - 1 (any number of them; where it ends inside a page, that page's
-    part). Those keys are read once a group, through its first row's table, the ones behind by each row; a listed row in no group
-    shares nothing. The bounds shape the launch, so that it can be captured while groups, shares and positions change on the device, and
-    must hold: shared[g] <= max_shared, position + 1 - shared[g] <= max_own, rows of a group <= max_group. `part_o` [n_rows, heads, parts,
-    head_dim] and `part_ml` [n_rows, heads, parts, 2] float32 are scratch, parts = attention_shared_parts(...); launches that may run
-    at once need scratch of their own. A row whose position is below 0 sees nothing and is zeros; rows that are not listed are left as
-    they are."""
+    """`attention_decode` for rows in groups that share a prefix: group g is the listed rows group_start[g] .. group_start[g + 1] - 1
+    (groups one behind the other, no row in two of them), whose keys 0 .. shared[g] - 1 are in the cache, in the same pages. Those keys
+    are read once a group, through its first row's table, and the ones behind by each row through its own (so a page in which the shared keys end
+    may be a copy in every row); a listed row in no group shares nothing. The bounds shape the launch, so that it can be captured while
+    groups, shares and positions change on the device, and must hold: shared[g] <= max_shared, position + 1 - shared[g] <= max_own, rows of
+    a group <= max_group. `part_o` [n_rows, heads, parts, head_dim] and `part_ml` [n_rows, heads, parts, 2] float32 are scratch, parts =
+    attention_shared_parts(...); launches that may run at once, and captured ones that may be replayed at once, need scratch of their own. Softmax
+    weights are rounded to bfloat16 before they meet the values. A row whose position is below 0 sees nothing and is zeros; rows that
+    are not listed are left as they are."""
     n, heads, head_dim, n_pages, kv_heads, page_size = _check_mfma(q, k_cache, v_cache, out)
     _here(q, "q")
     if window is not None and window < 1:

@@ -151,6 +151,18 @@ def test_flat_and_steep_scores(spread, scale):
     Batch([(400, [60, 3, 129])], 4, 2, 64, 32, seed=2, spread=spread).check(scale=scale)
 
 
+@pytest.mark.parametrize("seed", range(12))
+def test_batches_of_any_make(seed):
+    rng = np.random.default_rng(1000 + seed)
+    kv = int(rng.choice([1, 2, 3]))
+    groups = [(None if rng.random() < 0.2 else int(rng.integers(0, 400)), [int(b) for b in rng.integers(1, 200, rng.integers(1, 9))])
+              for _ in range(rng.integers(1, 6))]
+    groups = [g for g in groups if g[0] is not None] + [g for g in groups if g[0] is None]
+    b = Batch(groups, kv * int(rng.integers(1, 20)), kv, int(rng.choice([16, 32, 48, 64, 80, 96, 112, 128])),
+              int(rng.choice([16, 32, 64, 128])), seed=seed)
+    b.check(window=None if rng.random() < 0.6 else int(rng.integers(1, 300)), stretch=int(rng.choice([0, 100])))
+
+
 def test_a_long_prefix():
     Batch([(4500, [100, 600, 1])], 4, 2, 64, 64, seed=8).check()
 

@@ -41,11 +41,11 @@ def filters_of(rng, n, vocab):
 
 
 @pytest.mark.parametrize("vocab", [2, 5, 63, 1003, 4097, 16383, 16384, 50257, 65536, 130001])
-@pytest.mark.parametrize("values", ["normal", "steep", "quarters", "gaps"])
+@pytest.mark.parametrize("values", ["normal", "steep", "flat", "quarters", "gaps"])
 def test_picks(vocab, values):
     rng = np.random.default_rng(vocab)
     n = 24 if vocab < 20000 else 12
-    x = rng.standard_normal((n, vocab)).astype(np.float32) * (20.0 if values == "steep" else 2.0)
+    x = rng.standard_normal((n, vocab)).astype(np.float32) * {"steep": 20.0, "flat": 0.1}.get(values, 2.0)
     if values == "quarters":
         x = np.round(x * 4) / 4                                   # many ties
     if values == "gaps":
@@ -55,6 +55,19 @@ def test_picks(vocab, values):
     u = rng.integers(0, 1 << 24, n) / float(1 << 24)
     u[0], u[1], u[2] = 0.0, 1 - 2.0 ** -24, 1.0
     check(x.astype(np.float32), rng.uniform(0.3, 1.5, n), u, *filters_of(rng, n, vocab))
+
+
+@pytest.mark.parametrize("top_k,top_p,min_p", [(5000, 1.0, 0.0), (5000, 0.9, 0.0), (40000, 0.5, 0.01), (0, 0.97, 0.0), (0, 0.97, 0.02), (0, 0.97, 0.3),
+                                              (0, 1.0, 1e-4), (511, 0.99, 0.0), (513, 0.99, 0.0)])
+@pytest.mark.parametrize("steps", [0, 2, 64])
+def test_many_tokens_kept(top_k, top_p, min_p, steps):
+    """More than a list of 4,096 holds, by each filter and by two; logits in steps of 1 / steps, so that thousands tie at the border."""
+    rng = np.random.default_rng(steps + top_k)
+    n, vocab = 6, 50001
+    x = (rng.standard_normal((n, vocab)) * 0.8).astype(np.float32)
+    if steps:
+        x = np.round(x * steps) / steps
+    check(x.astype(np.float32), [0.9] * n, [0.0, 0.2, 0.5, 0.8, 0.999, 1.0], [top_k] * n, [top_p] * n, [min_p] * n)
 
 
 @pytest.mark.parametrize("vocab", [255, 16385, 65536])
