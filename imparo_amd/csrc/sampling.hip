@@ -274,17 +274,19 @@ extern "C" int imparo_sample_rows(const float* logits, const float* temperature,
 // One block a row, and what an instruction a logit costs is what the kernel costs (65,536 logits, 64 lanes a clock: 0.43 us each),
 // so the row is read few times (out of L2 after the first) and little is done a logit. First the largest; then how far down anything is
 // kept, as a number of bins, 2,048 over the 44 octaves that weigh anything: for min-p its own; for top-k the k-th largest of the threads'
-// own maxima, as k logits at least are no smaller; for top-p alone the bin of a histogram of weights where p of them is reached. The tokens above
-// that go into a list, four a thread at most, and border, ties and pick are found in the list alone, every
+// own maxima, as k logits at least are no smaller; for top-p alone the bin of a histogram of weights, 512 of them, where p of them is reached. The
+// tokens above that go into a list, four a thread at most, and border, ties and pick are found in the list alone, every
 // token compared with every other where they are few, else by histograms over nine bits of keys or indices at a time (list_find). A row
-// that keeps more under top-p lists the tokens of the border's bin only, sums up the ones above by the runs they are in, and picks in the
-// run that u falls in. What fits neither (large top-k, thousands of ties) is done over the row itself, pass by pass (pick_narrow).
+// that keeps more than a few under top-p lists the tokens of the border's bin only, has the sums of the ones above by the runs they are in (every wave has a
+// histogram of its run), and picks in the run that u falls in: one exponential a logit, and one for those of that run. What fits neither (large top-k, thousands of ties) is done over the row itself, pass by pass (pick_narrow).
 #define PICK_THREADS 1024          // of short rows too: 5 of 1,003 under top-k with 256 threads 13.1 us, so 9.9; 8 of 16,000 under top-p 53 and 24
 #define PICK_BINS 2048
 #define PICK_BITS 9                // bits of a key or an index that a search in the list settles at a time
 #define PICK_FEW 256               // tokens that are compared with one another instead
 #define PICK_EACH 4                // tokens of the list a thread has at most
 #define PICK_CUT 44
+#define PICK_RUNS (PICK_THREADS / WAVE)
+#define PICK_COARSE (PICK_BINS / 4)
 #define PICK_STEPS 512
 
 typedef unsigned long long u64;
@@ -331,7 +333,7 @@ __device__ __forceinline__ T wave_scan(T v) {                     // the sum ove
 }
 
 struct PickShared {
-    u64 hist[PICK_BINS];
+    u64 hist[PICK_RUNS * PICK_COARSE];      // (PICK_BINS of them where the runs do not have one each)
     u64 level[2][1 << PICK_BITS];     // used in turn: while one is read the other is cleared
     float list_x[PICK_EACH * PICK_THREADS];
     int list_index[PICK_EACH * PICK_THREADS];
@@ -506,6 +508,7 @@ __device__ __forceinline__ bool list_find(PickShared& sh, PickList& list, uint32
     constexpr int BINS = 1 << PICK_BITS, PER = BINS / WAVE;
     const int tid = threadIdx.x, lane = tid & (WAVE - 1);
     u64 above = 0, need = 0;
+    auto slot = [](uint32_t b) { return b % PER * WAVE + b / PER; };      // (a lane adds up PER neighbours: apart by as many as there are lanes, no two meet on a bank)
     for (bool first = true;; first = false) {
         const int bits = low == high ? 0 : 32 - __clz((int)(high - low)), shift = max(0, bits - PICK_BITS);
         u64* hist = sh.level[list.turn];
@@ -513,7 +516,7 @@ __device__ __forceinline__ bool list_find(PickShared& sh, PickList& list, uint32
 #pragma unroll
         for (int e = 0; e < PICK_EACH; ++e)
             if (e < list.n && list.counts[e] && list.ord[e] >= low && list.ord[e] <= high)
-                atomicAdd(&hist[(list.ord[e] - low) >> shift], list.counts[e]);
+                atomicAdd(&hist[slot((list.ord[e] - low) >> shift)], list.counts[e]);
         __syncthreads();
         if (tid >= WAVE) {
             for (int b = tid - WAVE; b < BINS; b += (int)blockDim.x - WAVE) sh.level[list.turn][b] = 0;
@@ -521,7 +524,7 @@ __device__ __forceinline__ bool list_find(PickShared& sh, PickList& list, uint32
             u64 bin[PER], mine = 0;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                bin[i] = hist[PER * lane + i];
+                bin[i] = hist[i * WAVE + lane];
                 mine += bin[i];
             }
             const u64 upto = wave_scan(mine);
@@ -630,6 +633,37 @@ __device__ __forceinline__ void pick_few(PickShared& sh, const PickWeights& weig
     }
 }
 
+// The same comparison for the border alone: of a list of at most PICK_FEW tokens, the last one in the order that is needed for `need` of their weights.
+// False where all of them are fewer.
+__device__ __forceinline__ bool pick_border(PickShared& sh, const PickWeights& weights, u64 need, PickSet& set) {
+    const int tid = threadIdx.x, n = sh.n_list;
+    const int bits = n <= WAVE ? 6 : 32 - __clz(n - 1);
+    const int i = tid & ((1 << bits) - 1), part = tid >> bits, parts = PICK_THREADS >> bits;
+    if (tid < n) {
+        sh.few_ord[tid] = (u64)~key_of(sh.list_x[tid]) << 32 | (uint32_t)sh.list_index[tid];
+        sh.few_weight[tid] = weights(sh.list_x[tid]);
+        sh.few_mass[0][tid] = 0;
+    }
+    if (tid == 0) sh.cut = -1;
+    __syncthreads();
+    u64 mass = 0;
+    const u64 ord = sh.few_ord[i];                                // (past the list: not used)
+    for (int j = part; j < n; j += parts) mass += sh.few_ord[j] < ord ? sh.few_weight[j] : 0;
+    if (i < n) atomicAdd(&sh.few_mass[0][i], mass);
+    __syncthreads();
+    if (tid < n) {
+        const u64 before = sh.few_mass[0][tid];
+        if (before < need && need <= before + sh.few_weight[tid]) {
+            sh.key_low = ~(uint32_t)(sh.few_ord[tid] >> 32);
+            sh.cut = (int)(uint32_t)sh.few_ord[tid];
+        }
+    }
+    __syncthreads();
+    if (sh.cut < 0) return false;
+    set = PickSet{sh.key_low, sh.cut};
+    return true;
+}
+
 // What is left to do in the list, in this order; the searches for ties only where not all of them stay
 enum { PICK_K, PICK_K_TIES, PICK_P, PICK_P_TIES, PICK_DRAW };
 
@@ -732,7 +766,7 @@ __device__ __forceinline__ void pick_in_runs(PickShared& sh, PickRow row, float 
     const u64 target = passed_at(u, total) - 1;
     u64 before = 0;
     int run = 0;
-    while (before + sh.waves[run] <= target) before += sh.waves[run++];
+    while (run < waves - 1 && before + sh.waves[run] <= target) before += sh.waves[run++];
     row.of_wave(run);
     auto four_of = [&](int c, u64 (&w)[4]) {
         float x[4];
@@ -753,7 +787,7 @@ __device__ __forceinline__ void pick_in_runs(PickShared& sh, PickRow row, float 
     __syncthreads();
     if (wave != 0) return;
     int c = 0;
-    while (before + sh.turns[c] <= target) before += sh.turns[c++];
+    while (c < row.turns - 1 && before + sh.turns[c] <= target) before += sh.turns[c++];
     u64 w[4];
     const u64 four = four_of(c, w), upto = wave_scan(four), past = __ballot(before + upto > target);
     if (lane == __ffsll((long long)past) - 1) {
@@ -800,7 +834,7 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
     float own_top = -INFINITY;                                    // the largest of this thread's
     auto largest = [&](const float (&x)[4]) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); };
     for (int i = tid; i < PICK_STEPS; i += THREADS) sh.table[i] = pick_table.v[i];
-    for (int b = tid; b < PICK_BINS; b += THREADS) sh.hist[b] = 0;
+    for (int b = tid; b < PICK_RUNS * PICK_COARSE; b += THREADS) sh.hist[b] = 0;
     for (int b = tid; b < 2 << PICK_BITS; b += THREADS) (&sh.level[0][0])[b] = 0;
     if (tid == 0) sh.n_list = 0;
     row.each<8>([&](const float (&x)[4], int) { own_top = fmaxf(own_top, largest(x)); });
@@ -845,33 +879,46 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
             if (sh.bin >= 0) limit = (float)(sh.bin + 1);
         }
     } else if (by_p) {
+        u64* run = sh.hist + wave * PICK_COARSE;
         row.each([&](const float (&x)[4], int) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float at = place(x[j]);
-                if (at < (float)PICK_BINS) atomicAdd(&sh.hist[(int)at], weights(x[j]));
+                if (at < (float)PICK_BINS) atomicAdd(&run[(int)at >> 2], weights(x[j]));
             }
         });
         __syncthreads();
-        pick_bin(sh, 0, share);
-        need_p = sh.need;
-        limit = (float)(sh.bin + 1);
-        // about how many tokens that is, from what the bins hold and a token of a bin weighs
-        float about = 0.f;
-        for (int i = 0; i < PICK_BINS / THREADS; ++i) {
-            const int b = tid * (PICK_BINS / THREADS) + i;
-            if (b <= sh.bin) about += (float)sh.hist[b] * __builtin_amdgcn_exp2f(((float)b + 0.5f) / BINS_AN_OCTAVE - (float)PICK_CUT);
+        u64 mine = 0;                                             // a thread's bin, over all runs
+        if (tid < PICK_COARSE)
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) mine += sh.hist[w * PICK_COARSE + tid];
+        const u64 upto = wave_scan(mine);
+        if (lane == WAVE - 1) sh.waves[wave] = upto;
+        __syncthreads();
+        u64 at = upto - mine, all = 0;
+        for (int w = 0; w < WAVES; ++w) {
+            at += w < wave ? sh.waves[w] : 0;
+            all += sh.waves[w];
         }
+        need_p = max((u64)1, (u64)ceil(share * (double)all));
+        if (at < need_p && need_p <= at + mine) {
+            sh.bin = tid;
+            sh.above = at;
+        }
+        // about how many tokens that is, from what the bins hold and a token of a bin weighs
+        float about = at < need_p ? (float)mine * __builtin_amdgcn_exp2f(((float)tid + 0.5f) * 4.f / BINS_AN_OCTAVE - (float)PICK_CUT) : 0.f;
         about = wave_sum(about);
         if (lane == 0) sh.tops[wave] = about;
         __syncthreads();
         about = 0.f;
         for (int w = 0; w < WAVES; ++w) about += sh.tops[w];
-        window = about > (float)ROOM && !by_m;                    // (of no bearing on the result: with too many for the list it is the other way after all)
+        window = about > 0.8f * (float)PICK_FEW;                  // (of no bearing on the result)
+        limit = 4.f * (float)(sh.bin + 1);
     }
-    const float border = (float)sh.bin;
+    // min-p's own border, as a number of bins: above its bin nothing is taken out, below it nothing kept (a hundredth aside, for roundings)
+    const float floor_place = (float)(-floor_y * (double)BINS_AN_OCTAVE);
     // (a token that min-p takes out need not be listed, unless top-p asks for the sum of the k largest)
-    if (by_m && !(by_k && by_p)) limit = fminf(limit, (float)(-floor_y * (double)BINS_AN_OCTAVE) * 1.0001f + 0.01f);
+    if (by_m && !(by_k && by_p)) limit = fminf(limit, floor_place * 1.0001f + 0.01f);
 
     // ---- the list
     auto enlist = [&](float x, int index) {
@@ -890,30 +937,35 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
             }
         });
         __syncthreads();
-        if (by_p && !by_k && sh.n_list > ROOM) {
+        if (by_p && !by_k && sh.n_list > PICK_FEW) {
             window = true;
             __syncthreads();
             if (tid == 0) sh.n_list = 0;
             __syncthreads();
         }
     }
+    // under top-p alone the list then has the tokens of one bin, top-p's or min-p's, whichever is the higher one: all above are kept
+    float border = 0.f;
+    bool by_border = false;                                       // (top-p's border is in that bin)
     if (window) {
-        limit = border + 1.f;
-        u64 sure = 0;                                             // what this wave's tokens above the border's bin weigh
+        const int floor_bin = (int)fmaxf(floor_place * 0.9999f - 0.01f, 0.f) >> 2, bin = by_m ? min(sh.bin, floor_bin) : sh.bin;
+        by_border = bin == sh.bin;
+        border = 4.f * (float)bin;
+        limit = border + 4.f;
+        if (by_m && bin == floor_bin) limit = fmaxf(limit, floor_place * 1.0001f + 0.01f);
         row.each([&](const float (&x)[4], int index) {
             if (place(largest(x)) < limit) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float at = place(x[j]);
-                    if (at < border) sure += weights(x[j]);
-                    else if (at < limit) enlist(x[j], index + j);
-                }
+                for (int j = 0; j < 4; ++j)
+                    if (place(x[j]) < limit && place(x[j]) >= border) enlist(x[j], index + j);
             }
         });
+        u64 sure = 0;                                             // what this wave's tokens above that bin weigh
+        for (int i = lane; i < bin; i += WAVE) sure += sh.hist[wave * PICK_COARSE + i];
         sure = wave_sum_u64(sure);
         if (lane == 0) sh.turns[wave] = sure;
         __syncthreads();
-        need_p -= sh.above;
+        if (by_border) need_p -= sh.above;
     }
     PickSet set{0u, INT_MAX};
     // (no listed token's key lies outside these)
@@ -928,9 +980,15 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
     int stage = by_k ? PICK_K : by_p ? PICK_P : PICK_DRAW;
     bool from_row = window || sh.n_list > ROOM;                   // the pick is made out of the row
     bool listed = sh.n_list <= ROOM;
-    if (!listed) {                                                // too many for the list as well: over the row itself
+    if (window && listed && sh.n_list <= PICK_FEW) {
+        if (by_border) pick_border(sh, weights, need_p, set);     // (else, and where fewer are there, all of the bin stay)
+        list.take(sh, weights, THREADS);
+    } else if (!listed) {                                         // too many for the list as well: over the row itself
         if (by_k) pick_narrow<true>(sh, row, set, top, bin_scale, weights, (u64)k, -1.0);
         if (by_p) pick_narrow<false>(sh, row, set, top, bin_scale, weights, 0, share);
+        stage = PICK_DRAW;
+    } else if (window && !by_border) {
+        list.take(sh, weights, THREADS);
     } else {
         list.take(sh, weights, THREADS);
         Found at;
@@ -990,10 +1048,9 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
     if (lowest > edge) {
         edge = lowest;
         cut = INT_MAX;
-        listed = false;                                           // (the sums above the window hold what min-p takes out)
     }
     auto kept = [&](float x, int index) { return x > edge || (x == edge && index <= cut); };
-    if (window && listed) {                                       // the runs' sums: what lies above the window, and what is kept of it
+    if (window && listed) {                                       // the runs' sums: what lies above the list's bin, and what is kept of it
         if (tid < WAVES) sh.waves[tid] = sh.turns[tid];
         __syncthreads();
 #pragma unroll
