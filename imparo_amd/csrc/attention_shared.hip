@@ -109,7 +109,10 @@ __device__ __forceinline__ bool moved_reference(float& m, float mx, float& corr,
 // ---- shared keys
 // A block's four waves take QW tiles of 32 queries and, for QW of 2, the two halves of a tile of keys. Bound by the exponentials with many queries (16 a lane
 // for 32 keys, a quarter of a lane's rate each, beside 2 ND products), by memory with few. Weights are rounded to bfloat16 for the second product, half a
-// step of 2^-8 each and of either sign; their sum takes them as they were.
+// step of 2^-8 each and of either sign; their sum takes them as they were. 32 heads by 8 of 64, 64 rows behind 32,768 keys (256 queries a kv
+// head): 44 us with the adding up of parts (47 with the two halves of a tile one after the other), 390 TFLOP/s; 24 by 8 of 128, four groups of
+// 16 rows behind 8,192 keys: 40 us, 3.3 TB/s, a tile's loads a block on their way. Not faster: the sums out of the matrix pipe (one more product a tile where the vector pipe waits as it
+// is), two tiles on their way in registers (they no longer fit), three blocks a CU (more parts to add up).
 template <int ND, int QW, bool PAGED>
 struct SharedBlock {
     static constexpr int D = ND * 16, DT = (ND + 1) / 2, THREADS = SHARED_WAVES * WAVE, KW = SHARED_WAVES / QW;
@@ -355,7 +358,10 @@ struct SharedBlock {
 // ---- a row's own keys
 // A wave by itself, with a tile of its own in LDS: one listed row, kv head, 16 of its queries (the heads of the kv head) and a part of the row's own keys.
 // Bound by memory; what a wave has to find out before its first key (four trips to memory one behind the other) weighs on every part, so parts are long
-// where there are waves enough.
+// where there are waves enough. Keys go past the caches, whose lines they would only push out (a tile's keys are whole lines; its values are half
+// lines, whose other half the next tile wants): 256 rows with 1,024 keys each on average, 8 kv heads of 64, 145 us through the caches, 122 so,
+// 4.4 TB/s, and 6 with rows of one length; the rest is the longest rows' end. Tiles of 64 keys (whole lines of values too) take the LDS that the
+// blocks of shared keys need: 115 us alone, but 64 rows behind 32,768 shared keys 48 -> 66.
 template <int ND, bool PAGED>
 struct OwnWave {
     static constexpr int D = ND * 16, NK = (ND + 1) / 2, LDK = D + 8, LDV = OWN_KEYS + 8, CH = D / 8;
