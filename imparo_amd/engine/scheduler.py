@@ -51,6 +51,7 @@ class Request:
     preemptions: int = 0
     arrival: int = 0
     drawn: int = 0                   # tokens sampled for it that count, read back or not
+    filtered: bool = False           # it asks for top-k, top-p or min-p
     # while its last sampled token has not been read back:
     unread: bool = False
     ended_by_length: bool = False    # that token is its last; it has left the engine already
@@ -138,7 +139,8 @@ class Scheduler:
     def add(self, request_id: Hashable, prompt: Sequence[int], params: SamplingParams) -> Request:
         if len(prompt) == 0:
             raise ValueError("a request needs at least one prompt token")
-        r = Request(request_id, list(prompt), params, pending=list(prompt), arrival=self._arrivals)
+        r = Request(request_id, list(prompt), params, pending=list(prompt), arrival=self._arrivals,
+                    filtered=params.filters != NO_FILTERS)
         self._arrivals += 1
         # a request the step function would refuse ends here, alone, instead of failing a step that
         # carries other requests (the reference answers such a request with an error of its own before
@@ -247,8 +249,9 @@ class Scheduler:
             return self._read_back()
         temps = [r.params.temperature for r in askers]
         unis = [uniform_for(r.params.seed, r.drawn) for r in askers]
-        filters = [r.params.filters for r in askers]
-        asked = (logits, temps, unis) if all(f == NO_FILTERS for f in filters) else (logits, temps, unis, filters)
+        asked = (logits, temps, unis)
+        if any(r.filtered for r in askers):
+            asked += ([r.params.filters for r in askers],)
         if self.pick_async is not None:
             pending = self.pick_async(*asked)
             out = self._read_back()          # the step before's tokens, while this step runs

@@ -208,6 +208,38 @@ def test_replays_follow_what_changes_on_the_device():
         assert bool(((out[:b.n].cpu().double() - want).abs() <= bound).all()), i
 
 
+def test_a_cache_of_more_than_2_to_32_elements():
+    """Pages at both ends of a cache whose last elements lie past 32 bits."""
+    b = Batch([(130, [40, 3, 90])], 8, 8, 128, 64, seed=12)
+    low = b.run()
+    n_pages = (1 << 32) // (8 * 64 * 128) + b.k.shape[0]
+    shift = n_pages - b.k.shape[0]
+    k = torch.empty(n_pages, 8, 64, 128, dtype=torch.bfloat16, device=DEV)
+    v = torch.empty(n_pages, 8, 128, 64, dtype=torch.bfloat16, device=DEV)
+    k[shift:], v[shift:] = b.k.to(DEV), b.v.to(DEV)
+    n, heads, dim = b.q.shape
+    bounds = dict(max_shared=b.max_shared, max_own=b.max_own, max_group=b.max_group)
+    parts = ops().attention_shared_parts(b.n, heads, 8, dim, 1, b.max_group, b.max_shared, b.max_own)
+    out = torch.zeros(n, heads * dim, dtype=torch.bfloat16, device=DEV)
+    table = np.where(b.table >= 0, b.table + shift, -1)
+    ops().attention_decode_shared(b.q.to(DEV), k, v, out, torch.empty(b.n, heads, parts, dim, device=DEV),
+                                  torch.empty(b.n, heads, parts, 2, device=DEV), ints(b.order), b.n, ints(b.group_start), ints(b.shared),
+                                  ints(np.arange(n)), ints(b.positions + [0]), ints(table), b.scale, None, **bounds)
+    assert torch.equal(out[:b.n].cpu(), low)                  # (the same work whatever the pages' numbers: the same bits)
+
+
+def test_two_streams_with_scratch_of_their_own():
+    a, b = Batch([(300, [30, 64, 5])], 8, 2, 64, 32, seed=3), Batch([(200, [3, 164, 50])], 8, 2, 64, 32, seed=4)
+    want = a.run(), b.run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got_b = b.run()
+    got_a = a.run()
+    torch.cuda.synchronize()
+    assert torch.equal(got_a, want[0]) and torch.equal(got_b, want[1])
+
+
 def test_refusals():
     b = Batch([(32, [4, 4])], 4, 2, 64, 32, seed=1)
     n, heads, dim = b.q.shape
