@@ -29,7 +29,7 @@
 #define SHARED_BLOCKS 512          // blocks that shared keys are cut for at most, two a CU
 #define OWN_KEYS 32                // a row's own keys of a tile
 #define OWN_MIN_SPLIT 64           // and of a part at least
-#define OWN_WAVES 3072             // waves that own keys are cut for
+#define OWN_WAVES (12 * 256)       // waves that own keys are cut for, twelve a CU
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));

@@ -320,12 +320,7 @@ __device__ __forceinline__ u64 moved(u64 v) {
     return ((u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false) << 32) |
            (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
 }
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float moved(float v) {
-    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, ROWS, 0xf, false));
-}
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {                     // the sum over the lanes up to and with this one
+__device__ __forceinline__ u64 wave_scan(u64 v) {                 // the sum over the lanes up to and with this one
     v += moved<0x111, 0xf>(v);                                    // row_shr:1, 2, 4, 8
     v += moved<0x112, 0xf>(v);
     v += moved<0x114, 0xf>(v);

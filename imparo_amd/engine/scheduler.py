@@ -152,6 +152,11 @@ class Scheduler:
             if bad is not None:
                 self._finish(r, f"error: token id {bad!r} is outside the vocabulary of {vocab}")
                 return r
+            if r.filtered:
+                from ..kernels.ops import PICK_MAX_VOCAB
+                if vocab > PICK_MAX_VOCAB:
+                    self._finish(r, f"error: top_k, top_p and min_p take a vocabulary of at most {PICK_MAX_VOCAB}, not {vocab}")
+                    return r
         limit = getattr(self.engine, "max_position", None)
         if limit is not None and len(r.prompt) + max(params.max_tokens, 1) - 1 > limit:
             self._finish(r, f"error: {len(r.prompt)} prompt tokens and {params.max_tokens} new ones pass the "

@@ -39,3 +39,19 @@ def test_the_scheduler_hands_filters_over_only_where_a_request_has_some():
     s.add("c", [1, 2], SamplingParams(max_tokens=1, top_k=4, min_p=0.1))
     s.run()
     assert seen == [([(0, 1.0, 0.0), (4, 1.0, 0.1)],)]
+
+
+def test_a_vocabulary_that_is_not_filtered_ends_the_request_alone():
+    from test_scheduler import make
+    from imparo_amd.kernels.ops import PICK_MAX_VOCAB
+    from imparo_amd.sampling.sampler import SamplingParams
+    eng, s = make(n_pages=64)
+    plain_pick = s.pick
+    s.pick = lambda logits, t, u, *more: plain_pick(logits, t, u)
+    eng.vocab_size = PICK_MAX_VOCAB
+    assert s.add("a", [1, 2], SamplingParams(max_tokens=1, top_k=4)).finish_reason == ""
+    eng.vocab_size = PICK_MAX_VOCAB + 1
+    assert s.add("b", [1, 2], SamplingParams(max_tokens=1, top_k=4)).finish_reason.startswith("error: top_k")
+    assert s.add("c", [1, 2], SamplingParams(max_tokens=1)).finish_reason == ""
+    s.run()
+    assert s.finished["a"].finish_reason == s.finished["c"].finish_reason == "length"
