@@ -274,14 +274,14 @@ extern "C" int imparo_sample_rows(const float* logits, const float* temperature,
 // One block a row, and what an instruction a logit costs is what the kernel costs (65,536 logits, 64 lanes a clock: 0.43 us each),
 // so the row is read few times (out of L2 after the first) and little is done a logit. First the largest; then how far down anything is
 // kept, as a number of bins, 2,048 over the 44 octaves that weigh anything: for min-p its own; for top-k the k-th largest of the threads'
-// own maxima, as k logits at least are no smaller; for top-p alone the bin of a histogram of weights, 512 of them, where p of them is reached. The
+// own maxima, as k logits at least are no smaller; for top-p alone the bin of a histogram of weights, 512 of them as fine as the row allows, where p of them is reached. The
 // tokens above that go into a list, four a thread at most, and border, ties and pick are found in the list alone, every
 // token compared with every other where they are few, else by histograms over nine bits of keys or indices at a time (list_find). A row
 // that keeps more than a few under top-p lists the tokens of the border's bin only, has the sums of the ones above by the runs they are in (every wave has a
 // histogram of its run), and picks in the run that u falls in: one exponential a logit, and one for those of that run. What fits neither (large top-k, thousands of ties) is done over the row itself, pass by pass (pick_narrow).
-// Measured, a row a block: one of 65,536 under top-k (and top-p) 12.3 us, under min-p 10.4, under top-p 24 where hardly any are kept, 30 with hundreds,
-// 41 with thousands (of which the largest 6, weights and their histogram 14, the border's tokens 5 to 9, border and pick 4 to 11); 64 rows
-// under top-k and top-p 15; 256 rows of 130,001 of all kinds 85, under top-k 46.
+// Measured, a row a block: one of 65,536 under top-k (and top-p) 12.3 us, under min-p 10.4, under top-p 24 where hardly any are kept, 28 with hundreds,
+// 34 to 39 with thousands (of which the largest 6, weights and their histogram 13, the border's tokens 5 to 9, border and pick 4 to 11); 64 rows
+// under top-k and top-p 15; 256 rows of 130,001 of all kinds 82, under top-k 46.
 #define PICK_THREADS 1024          // of short rows too: 5 of 1,003 under top-k with 256 threads 13.1 us, so 9.9; 8 of 16,000 under top-p 53 and 24
 #define PICK_BINS 2048
 #define PICK_BITS 9                // bits of a key or an index that a search in the list settles at a time
@@ -335,9 +335,9 @@ struct PickShared {
     u64 level[2][1 << PICK_BITS];     // used in turn: while one is read the other is cleared
     float list_x[PICK_EACH * PICK_THREADS];
     int list_index[PICK_EACH * PICK_THREADS];
-    double table[PICK_STEPS];         // 2^(i / PICK_STEPS)
+    double table[PICK_STEPS];         // 2^(PICK_CUT + i / PICK_STEPS)
     u64 waves[16], turns[132];
-    float tops[16];
+    float tops[16], sums[16];
     u64 few_ord[PICK_FEW], few_weight[PICK_FEW], few_mass[2][PICK_FEW], few_sum[2];
     int few_rank[PICK_FEW];
     u64 above, inside, need;          // of the bin where the sum is reached: what lies above it, what it holds; what is asked for
@@ -346,7 +346,7 @@ struct PickShared {
     uint32_t key_low, key_high;
 };
 
-// 2^(i / PICK_STEPS): e^z as its power series up to z^17 / 17!, z < 0.7, below a tenth of a float64's step
+// 2^(PICK_CUT + i / PICK_STEPS): e^z as its power series up to z^17 / 17!, z < 0.7, below a tenth of a float64's step
 struct PickTable {
     double v[PICK_STEPS];
     constexpr PickTable() : v() {
@@ -354,7 +354,7 @@ struct PickTable {
             const double z = 0.69314718055994530942 * i / PICK_STEPS;
             double sum = 1.0;
             for (int n = 17; n > 0; --n) sum = 1.0 + sum * z / n;
-            v[i] = sum;
+            v[i] = sum * (double)(1ull << PICK_CUT);
         }
     }
 };
@@ -362,7 +362,7 @@ static __device__ const PickTable pick_table = PickTable();
 
 // Weights of a row: 2^y 2^44 to the nearest integer, y = (x - top) c1 <= 0, for y above -45 (what is asked about lies in one of the bins).
 // y 512 = n + f with n whole, 2^(n / 512) out of a table and an exponent, and 2^(f / 512), |f| <= 1/2, from its power series, cut where the next term
-// is below 2^-46; rounded by an addition of 2^52, whose low bits then are the integer.
+// is below 2^-46; rounded with the addition of 2^52, whose low bits then are the integer.
 struct PickWeights {
     static_assert(PICK_STEPS == 1 << 9, "the shift below");
     double top, c;                    // c1 PICK_STEPS
@@ -373,8 +373,9 @@ struct PickWeights {
         const int n = __double2loint(t);
         double p = fma(f, L * L * L / 6, L * L / 2);
         p = fma(f, p, L);
-        p = fma(f, p, 1.0) * table[n & (PICK_STEPS - 1)];
-        const double v = __hiloint2double(__double2hiint(p) + (((n >> 9) + PICK_CUT) << 20), __double2loint(p)) + 4503599627370496.0;
+        p = fma(f, p, 1.0);
+        const double step = table[n & (PICK_STEPS - 1)];
+        const double v = fma(p, __hiloint2double(__double2hiint(step) + (int)((uint32_t)(n & -PICK_STEPS) << 11), __double2loint(step)), 4503599627370496.0);
         return (u64)__double_as_longlong(v) & 0xFFFFFFFFFFFFFull;
     }
     __device__ __forceinline__ double octaves(float x) const { return ((double)x - top) * c * (1.0 / PICK_STEPS); }
@@ -836,11 +837,18 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
     for (int b = tid; b < 2 << PICK_BITS; b += THREADS) (&sh.level[0][0])[b] = 0;
     if (tid == 0) sh.n_list = 0;
     row.each<8>([&](const float (&x)[4], int) { own_top = fmaxf(own_top, largest(x)); });
-    float top = wave_max(own_top);
-    if (lane == 0) sh.tops[wave] = top;
+    float top = wave_max(own_top), mean_top = wave_sum(own_top);
+    if (lane == 0) {
+        sh.tops[wave] = top;
+        sh.sums[wave] = mean_top;
+    }
     __syncthreads();
+    mean_top = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sh.tops[w]);
+    for (int w = 0; w < WAVES; ++w) {
+        top = fmaxf(top, sh.tops[w]);
+        mean_top += sh.sums[w];
+    }
     if (!(top < INFINITY) || !(top > -INFINITY)) {                // an infinite logit takes it, or there is none to take
         if (tid < sample_threads(vocab)) sample_row(row_at, 0.f, u, out + r, vocab, sample_threads(vocab));
         return;
@@ -851,7 +859,21 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
     const double floor_y = by_m ? fmax(-(double)PICK_CUT, log2((double)fminf(mp, 1.f))) : -(double)PICK_CUT;
     // bins an octave, and a unit of the logit: a logit d below the top is in bin d bin_scale
     constexpr float BINS_AN_OCTAVE = (float)PICK_BINS / PICK_CUT;
-    const float bin_scale = BINS_AN_OCTAVE * (float)c1;
+    const float whole_scale = BINS_AN_OCTAVE * (float)c1;
+    float bin_scale = whole_scale, finer = 1.f;                   // (bin_scale / whole_scale)
+    if (by_p && !by_k) {
+        // Under top-p alone the bins are as fine as leaves the last one few: where a row is nearly flat, lanes that add to one bin wait for one another,
+        // and its border's bin is long: 130,001 logits with a deviation of 0.2, T = 1 and p = 0.5 take 225 us with bins over all octaves, 63 so. Six times the way
+        // from the largest logit to the mean of the threads' largest ones ends, in a row like noise, four deviations below the middle (four times: two, where 256
+        // such rows had one or another whose border was in the last bin, 120 us more). What lies behind the last bin counts as in it; of no bearing on the result
+        const float range = 6.f * (top - mean_top * (1.f / THREADS));
+        if (range * whole_scale < (float)PICK_BINS) {
+            finer = fminf(fminf((float)PICK_BINS / (range * whole_scale), 1024.f), 1.0e38f / whole_scale);    // (a whole_scale of 0, T infinite: 1024)
+            bin_scale = whole_scale * finer;
+        }
+    }
+    const float far = (float)PICK_BINS * finer;                   // so many bins are PICK_CUT octaves
+    constexpr int LAST = PICK_COARSE - 1;
     auto place = [&](float x) { return (top - x) * bin_scale; };
 
     // ---- how far down the list has to reach: `limit`, a number of bins
@@ -882,7 +904,7 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float at = place(x[j]);
-                if (at < (float)PICK_BINS) atomicAdd(&run[(int)at >> 2], weights(x[j]));
+                if (at < far) atomicAdd(&run[min((int)at >> 2, LAST)], weights(x[j]));
             }
         });
         __syncthreads();
@@ -904,17 +926,17 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
             sh.above = at;
         }
         // about how many tokens that is, from what the bins hold and a token of a bin weighs
-        float about = at < need_p ? (float)mine * __builtin_amdgcn_exp2f(((float)tid + 0.5f) * 4.f / BINS_AN_OCTAVE - (float)PICK_CUT) : 0.f;
+        float about = at < need_p ? (float)mine * __builtin_amdgcn_exp2f(((float)tid + 0.5f) * 4.f / (BINS_AN_OCTAVE * finer) - (float)PICK_CUT) : 0.f;
         about = wave_sum(about);
         if (lane == 0) sh.tops[wave] = about;
         __syncthreads();
         about = 0.f;
         for (int w = 0; w < WAVES; ++w) about += sh.tops[w];
         window = about > 0.8f * (float)PICK_FEW;                  // (of no bearing on the result)
-        limit = 4.f * (float)(sh.bin + 1);
+        limit = sh.bin < LAST ? 4.f * (float)(sh.bin + 1) : far;
     }
     // min-p's own border, as a number of bins: above its bin nothing is taken out, below it nothing kept (a hundredth aside, for roundings)
-    const float floor_place = (float)(-floor_y * (double)BINS_AN_OCTAVE);
+    const float floor_place = (float)(-floor_y * (double)BINS_AN_OCTAVE) * finer;
     // (a token that min-p takes out need not be listed, unless top-p asks for the sum of the k largest)
     if (by_m && !(by_k && by_p)) limit = fminf(limit, floor_place * 1.0001f + 0.01f);
 
@@ -944,15 +966,20 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
     }
     // under top-p alone the list then has the tokens of one bin, top-p's or min-p's, whichever is the higher one: all above are kept
     float border = 0.f;
+    // (no listed token lies outside these)
+    auto highest_listed = [&]() { return fminf(top, top - border / bin_scale * 0.9999f + fabsf(top) * 1.0e-5f); };
+    auto lowest_listed = [&]() { return top - limit / bin_scale * 1.0001f - fabsf(top) * 1.0e-5f; };
     bool by_border = false;                                       // (top-p's border is in that bin)
     if (window) {
-        const int floor_bin = (int)fmaxf(floor_place * 0.9999f - 0.01f, 0.f) >> 2, bin = by_m ? min(sh.bin, floor_bin) : sh.bin;
+        const int floor_bin = min((int)fmaxf(floor_place * 0.9999f - 0.01f, 0.f) >> 2, LAST), bin = by_m ? min(sh.bin, floor_bin) : sh.bin;
         by_border = bin == sh.bin;
         border = 4.f * (float)bin;
-        limit = border + 4.f;
+        limit = bin < LAST ? border + 4.f : far;
         if (by_m && bin == floor_bin) limit = fmaxf(limit, floor_place * 1.0001f + 0.01f);
+        // (a few of many: four at a time by their distance from the middle of what may be listed)
+        const float low = 0.5f * lowest_listed(), high = 0.5f * highest_listed(), middle = low + high, reach = high - low + (fabsf(low) + fabsf(high)) * 1.0e-5f;
         row.each([&](const float (&x)[4], int index) {
-            if (place(largest(x)) < limit) {
+            if (fminf(fminf(fabsf(x[0] - middle), fabsf(x[1] - middle)), fminf(fabsf(x[2] - middle), fabsf(x[3] - middle))) <= reach) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (place(x[j]) < limit && place(x[j]) >= border) enlist(x[j], index + j);
@@ -966,9 +993,7 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
         if (by_border) need_p -= sh.above;
     }
     PickSet set{0u, INT_MAX};
-    // (no listed token's key lies outside these)
-    const uint32_t key_high = window ? key_of(fminf(top, top - border / bin_scale * 0.9999f + fabsf(top) * 1.0e-5f)) : key_of(top);
-    const uint32_t key_low = key_of(top - limit / bin_scale * 1.0001f - fabsf(top) * 1.0e-5f);
+    const uint32_t key_high = key_of(highest_listed()), key_low = key_of(lowest_listed());
     if (!window && sh.n_list <= PICK_FEW) {
         pick_few<THREADS>(sh, weights, k, share, by_k, by_p, need_p, floor_y, u, out + r);
         return;
@@ -982,8 +1007,8 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
         if (by_border) pick_border(sh, weights, need_p, set);     // (else, and where fewer are there, all of the bin stay)
         list.take(sh, weights, THREADS);
     } else if (!listed) {                                         // too many for the list as well: over the row itself
-        if (by_k) pick_narrow<true>(sh, row, set, top, bin_scale, weights, (u64)k, -1.0);
-        if (by_p) pick_narrow<false>(sh, row, set, top, bin_scale, weights, 0, share);
+        if (by_k) pick_narrow<true>(sh, row, set, top, whole_scale, weights, (u64)k, -1.0);
+        if (by_p) pick_narrow<false>(sh, row, set, top, whole_scale, weights, 0, share);
         stage = PICK_DRAW;
     } else if (window && !by_border) {
         list.take(sh, weights, THREADS);

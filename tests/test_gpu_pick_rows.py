@@ -70,6 +70,29 @@ def test_many_tokens_kept(top_k, top_p, min_p, steps):
     check(x.astype(np.float32), [0.9] * n, [0.0, 0.2, 0.5, 0.8, 0.999, 1.0], [top_k] * n, [top_p] * n, [min_p] * n)
 
 
+@pytest.mark.parametrize("make", ["noise", "high", "half", "spike", "pit", "slope"])
+@pytest.mark.parametrize("spread", [1e-5, 0.01, 0.2, 1.0])
+def test_rows_that_are_nearly_flat(spread, make):
+    """Nearly everything counts for something, and top-p's border lies far down: rows far from zero, with masked halves, with one logit far above
+    or below the others, with a long even slope."""
+    rng = np.random.default_rng(int(spread * 1e6))
+    n, vocab = 8, 40003
+    x = rng.standard_normal((n, vocab)) * spread
+    if make == "high":
+        x += 500.0
+    if make == "half":
+        x[:, ::2] = -np.inf
+    if make == "spike":
+        x[:, 17] += 4.0
+    if make == "pit":
+        x[:, 17] -= 1e6
+    if make == "slope":
+        x = np.linspace(0.0, spread, vocab)[None].repeat(n, 0)
+    top_p = [0.01, 0.3, 0.95, 0.999, 0.99999, 0.3, 0.95, 0.999]
+    check(x.astype(np.float32), [1.0, 0.7, 1.0, 1.3, 1.0, 0.7, 1.0, 1.3], [0.1, 0.9, 0.5, 0.99, 1.0, 0.0, 0.7, 0.3], [0] * n, top_p,
+          [0.0] * 5 + [0.5, 0.9, 0.01])
+
+
 @pytest.mark.parametrize("vocab", [255, 16385, 65536])
 def test_equal_logits_count_in_the_order_of_ids(vocab):
     """All logits alike (as -0 and 0 are): k of them are the first k, a share p of them the first ceil(p n)."""
@@ -93,6 +116,9 @@ def test_extreme_logits_and_temperatures():
     x[5] = x[5] * 1e-3 + 1e6
     temperature = [1.0, 1.0, 1.0, 1e28, 1.0, 1e-3, 1e-40, 1e30, 0.0, -1.0]
     check(x, temperature, [0.3] * 10, [40] * 10, [0.9] * 10, [0.0] * 10)
+    temperature[8:] = [float("inf"), 3.4e38]
+    for k, p, m in ((0, 0.9, 0.0), (0, 0.9, 0.01), (0, 1.0, 0.01), (600, 1.0, 0.0)):
+        check(x, temperature, [0.3] * 10, [k] * 10, [p] * 10, [m] * 10)
 
 
 @pytest.mark.parametrize("vocab", [1003, 16384, 65536])
