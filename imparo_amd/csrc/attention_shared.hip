@@ -319,6 +319,39 @@ struct SharedBlock {
             }
         }
         l += lane_xor<32>(l);
+        // A value that is infinite or NaN at a key that a query does not see (it lies further back, or ahead of its window) goes into the product
+        // with a weight of 0, and makes NaN of the query's sums all the same. That is noticed here, and these sums are made anew out of the keys
+        // that the query sees. (0.3 us of a call that takes 10; to look at the values as they are read takes registers that the loop has not got)
+        float zeros = 0.f;                                        // (0 as long as all are finite)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (32 * dt + 8 * (r >> 2) < D) zeros += o[dt][r] * 0.f;
+        if (__builtin_expect(valid && zeros != 0.f && fabsf(l) < INFINITY, 0)) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+            const float from = m == -INFINITY ? 0.f : m;
+            const bf16_t* one_q = a.q + ((size_t)t * a.heads + head) * D;
+            for (int key = lo; key <= hi; ++key) {
+                if (KW > 1 && (key >> 5 & 1) != kw) continue;
+                const size_t first = ((a_page(a, table[key >> a.page_shift]) * a.kv_heads + kvh) << a.page_shift) * D;
+                const int slot = key & (page_size - 1);
+                float dot = 0.f;
+#pragma unroll 1
+                for (int d = 0; d < D; ++d) dot = fmaf(bf16_to_f32(one_q[d]), bf16_to_f32(a.k[first + (size_t)slot * D + d]), dot);
+                const float p = bf16_to_f32(f32_to_bf16(__builtin_amdgcn_exp2f(fmaf(a.flip ? -dot : dot, a.scale, -from))));
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int d = 32 * dt + 8 * (r >> 2);
+                        if (d < D) o[dt][r] = fmaf(p, bf16_to_f32(a.v[first + ((size_t)(d + 4 * h + (r & 3)) << a.page_shift) + slot]), o[dt][r]);
+                    }
+            }
+        }
         if constexpr (KW > 1) {                                   // the waves of the second halves hand over to those of the first
             float* meet = reinterpret_cast<float*>(lds) + qw * (DT * 16 + 2) * WAVE + lane;
             __syncthreads();

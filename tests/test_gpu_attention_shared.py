@@ -145,6 +145,25 @@ def test_windows(window):
     Batch([(290, [1, 40, 128, 300]), (20, [3, 3])], 4, 2, 64, 32, seed=window).check(window=window)
 
 
+@pytest.mark.parametrize("heads,kv,dim,page", [(4, 2, 64, 32), (4, 2, 48, 64), (48, 1, 64, 64), (48, 1, 128, 16), (70, 2, 80, 128)])
+@pytest.mark.parametrize("groups,window", [([(210, [-150, -60, 4, 30])], None), ([(290, [1, 40, 128])], 100), ([(290, [-200, -120, 3, 200])], 150)])
+@pytest.mark.parametrize("scale", [None, -0.2])
+def test_values_that_are_not_finite_reach_only_rows_that_see_them(groups, window, scale, heads, kv, dim, page):
+    """Among the shared keys, where some rows of a group see what others do not: an infinity, then one of the other sign and a NaN."""
+    b = Batch(groups, heads, kv, dim, page, seed=dim)
+    table = b.tables[int(np.argmax(b.positions))]
+    for key, d, value in ((100, 1, float("inf")), (110, 4, float("-inf")), (190, 2, float("nan")), (200, 3, float("-inf")), (206, 3, float("inf"))):
+        if key < groups[0][0] // page * page:
+            b.v[table[key // page], :, d, key % page] = value
+    got = b.run(window, scale=scale).double()
+    want, bound = plain.attend(b.q[:b.n], b.k, b.v, b.tables, b.positions, scale or b.scale, window)
+    fine = want.isfinite()
+    assert not fine.all() and fine.view(b.n, heads, dim).all(dim=2).any()          # rows of either kind
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[want.isinf()], want[want.isinf()])
+    over = (got - want).abs()[fine] - bound[fine]
+    assert bool((over <= 0).all()), float(over.max())
+
+
 @pytest.mark.parametrize("spread,scale", [(0.0, None), (30.0, None), (1.5, -0.2), (1.5, 1e-3)])
 def test_flat_and_steep_scores(spread, scale):
     """Queries of zero (all keys alike), scores far apart (the reference of the exponentials moves from tile to tile), and scales of either sign."""
