@@ -835,20 +835,26 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
     for (int i = tid; i < PICK_STEPS; i += THREADS) sh.table[i] = pick_table.v[i];
     for (int b = tid; b < PICK_RUNS * PICK_COARSE; b += THREADS) sh.hist[b] = 0;
     for (int b = tid; b < 2 << PICK_BITS; b += THREADS) (&sh.level[0][0])[b] = 0;
-    if (tid == 0) sh.n_list = 0;
+    if (tid == 0) {
+        sh.n_list = 0;
+        sh.bin = PICK_COARSE - 1;                                 // (found anew under top-p: the largest logit weighs 2^PICK_CUT, in bin 0)
+        sh.above = 0;
+    }
     row.each<8>([&](const float (&x)[4], int) { own_top = fmaxf(own_top, largest(x)); });
-    float top = wave_max(own_top), mean_top = wave_sum(own_top);
+    float top = wave_max(own_top);
+    // how far the threads' largest logits lie below the row's, added up: distances, none of them negative however it rounds (a mean of the logits
+    // themselves may come out above the largest where all are alike). Infinite or NaN where a thread has none, or the sum is out of range
+    const float below_wave = wave_sum(top - own_top);
     if (lane == 0) {
         sh.tops[wave] = top;
-        sh.sums[wave] = mean_top;
+        sh.sums[wave] = below_wave;
     }
     __syncthreads();
-    mean_top = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        top = fmaxf(top, sh.tops[w]);
-        mean_top += sh.sums[w];
-    }
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sh.tops[w]);
+    float below = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) below += sh.sums[w] + WAVE * (top - sh.tops[w]);
     if (!(top < INFINITY) || !(top > -INFINITY)) {                // an infinite logit takes it, or there is none to take
         if (tid < sample_threads(vocab)) sample_row(row_at, 0.f, u, out + r, vocab, sample_threads(vocab));
         return;
@@ -866,7 +872,7 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
         // and its border's bin is long: 130,001 logits with a deviation of 0.2, T = 1 and p = 0.5 take 225 us with bins over all octaves, 63 so. Six times the way
         // from the largest logit to the mean of the threads' largest ones ends, in a row like noise, four deviations below the middle (four times: two, where 256
         // such rows had one or another whose border was in the last bin, 120 us more). What lies behind the last bin counts as in it; of no bearing on the result
-        const float range = 6.f * (top - mean_top * (1.f / THREADS));
+        const float range = 6.f / THREADS * below;                // (neither infinite nor NaN is less than what it is compared with)
         if (range * whole_scale < (float)PICK_BINS) {
             finer = fminf(fminf((float)PICK_BINS / (range * whole_scale), 1024.f), 1.0e38f / whole_scale);    // (a whole_scale of 0, T infinite: 1024)
             bin_scale = whole_scale * finer;

@@ -221,3 +221,21 @@ def test_generate_draws_among_the_likeliest(loud_model_dirs):
     assert some != free and some != greedy
     assert generate(d, prompts[:1], max_tokens=8, dtype="float32", page_size=8, temperature=5.0, seed=3, top_k=3) == some[:1]
     assert generate(d, prompts, max_tokens=8, dtype="float32", page_size=8, temperature=5.0, seed=3, top_k=3, overlap=False) == some
+
+
+@pytest.mark.parametrize("vocab", [16385, 65536])
+@pytest.mark.parametrize("level", [0.1, 1.1, 4.9, -11.762, 1e36])
+def test_rows_whose_largest_logits_are_all_alike(level, vocab):
+    """Every thread's largest logit is the row's, a number whose multiples round (or overflow): constant rows under top-p, alone and with
+    min-p, and constant rows of which a part is masked, hardly likely or far below; each behind a row of another kind, with other bins."""
+    rng = np.random.default_rng(vocab)
+    rows = []
+    for rest in (None, -np.inf, level - 60, level - 1e4):
+        x = np.full(vocab, level)
+        if rest is not None:
+            x[rng.random(vocab) < 0.3] = rest
+        rows += [rng.standard_normal(vocab) * 2, x]
+    x = np.stack(rows).astype(np.float32)
+    n = len(rows)
+    for p, m in ((0.5, 0.0), (0.95, 0.3), (1e-6, 0.0), (1.0 - 2.0 ** -20, 1.0)):
+        check(x, [1.0, 0.7] * (n // 2), [0.3, 0.0, 0.9, 0.3, 0.1, 0.7, 0.5, 0.999], [0] * n, [0.9, p] * (n // 2), [0.0, m] * (n // 2))
