@@ -562,16 +562,18 @@ __global__ __launch_bounds__(SHARED_WAVES * WAVE) void k_attn_shared_merge(Share
     const int pre = min((keys + a.pre_split - 1) / a.pre_split, a.n_pre);
     const int own = keys < end_all ? min((end_all - (keys & ~(OWN_KEYS - 1)) + a.own_split - 1) / a.own_split, a.n_own) : 0;
     auto there = [&](int k) { return k < pre || (k >= a.n_pre && k < a.n_pre + own); };
+    // A part in which the row sees nothing is -inf, 0 and zeros; one whose scores are all NaN has no reference either, but a NaN for a sum, and weighs
+    // NaN. What a part holds counts even where its weight vanishes beside the others': NaN times 0 is NaN.
     float top = there(lane) ? ml.x : -INFINITY;
     for (int k = lane + WAVE; k < parts; k += WAVE) top = fmaxf(top, there(k) ? a.part_ml[2 * (base + k)] : -INFINITY);
     top = wave_max(top);
     float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
     for (int k0 = 0; k0 < parts; k0 += WAVE) {                   // lane j holds the weight of part k0 + j
-        float w = 0.f;
+        float w = -1.f;                                           // (no such part: scratch that nobody wrote)
         if (there(k0 + lane)) {
             if (k0) ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (base + k0 + lane));
-            w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
-            sum += w > 0.f ? ml.y * w : 0.f;
+            w = ml.x == -INFINITY ? ml.y : __builtin_amdgcn_exp2f(ml.x - top);
+            sum += ml.y * w;
         }
         const int here = min(WAVE, parts - k0);
         for (int j0 = 0; j0 < here; j0 += GROUP * side) {
@@ -580,7 +582,7 @@ __global__ __launch_bounds__(SHARED_WAVES * WAVE) void k_attn_shared_merge(Share
             for (int j = 0; j < GROUP; ++j) {
                 const int k = j0 + j * side + sub;
                 const float wk = __shfl(w, min(k, WAVE - 1), WAVE);
-                const bool on = works && k < here && wk > 0.f;
+                const bool on = works && k < here && !(wk < 0.f);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[e] += on ? v[j][e] * wk : 0.f;
             }
@@ -592,7 +594,7 @@ __global__ __launch_bounds__(SHARED_WAVES * WAVE) void k_attn_shared_merge(Share
 #pragma unroll
         for (int j = 0; j < 4; ++j) total[j] += __shfl(acc[j], lane % lanes_a_part + k * lanes_a_part, WAVE);
     if (sub != 0) return;
-    const float inv = sum > 0.f ? 1.0f / sum : 0.f;              // a row that sees nothing is zeros
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;             // a row that sees nothing is zeros
     uint2 packed;
     packed.x = f32x2_to_bf16x2(total[0] * inv, total[1] * inv);
     packed.y = f32x2_to_bf16x2(total[2] * inv, total[3] * inv);

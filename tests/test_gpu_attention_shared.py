@@ -1,4 +1,6 @@
 """Decode attention of rows that share a prefix against the plain form in 64 bits."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -280,3 +282,39 @@ def test_refusals():
     out = torch.full_like(good["out"], 3.0)
     ops().attention_decode_shared(**{**good, "out": out, "n_rows": 0})
     assert bool((out == 3.0).all())
+
+
+@pytest.mark.parametrize("heads,kv,dim,page", [(4, 2, 64, 32), (4, 2, 48, 64), (48, 1, 128, 16), (70, 2, 80, 128)])
+@pytest.mark.parametrize("where", ["query", "key alone", "key among others", "key far down", "infinite key", "value far down"])
+@pytest.mark.parametrize("scale", [None, -0.2])
+def test_what_is_not_a_number_in_what_a_row_sees(where, scale, heads, kv, dim, page):
+    """In a query, in keys (the only one of a part, one of many, one whose part weighs nothing beside another) and in a value whose part
+    weighs nothing: no finite result where the plain form has none, and no other row touched."""
+    b = Batch([(290, [1, 40, 1]), (40, [3, 2]), (None, [70])], heads, kv, dim, page, seed=dim)
+    r, nan = int(b.order[0]), float("nan")
+    place = lambda key: (b.tables[r][key // page], key % page)
+    if where == "query":
+        b.q[r, 1, 5] = nan
+    if where == "key alone":
+        p, s = place(290)
+        b.k[p, :, s] = nan
+    if where == "key among others":
+        p, s = place(100)
+        b.k[p, 0, s, 7] = nan
+    if where == "infinite key":                                # (an infinite score, or one of minus infinity, as the query's sign has it)
+        p, s = place(100)
+        b.k[p, :, s, 3] = float("inf")
+    if where.endswith("far down"):                             # all of the row's weight in the first head on its last key
+        p, s = place(290)
+        b.k[p, 0, s] = 30.0 * torch.sign(b.q[r, 0]) * (-1 if scale else 1)
+        p, s = place(5)
+        if where == "key far down":
+            b.k[p, 0, s, 7] = nan
+        else:
+            b.v[p, 0, 2, s] = nan
+    got = b.run(scale=scale).double()
+    want, bound = plain.attend(b.q[:b.n], b.k, b.v, b.tables, b.positions, scale or b.scale)
+    assert want.isnan().any() and not want.isnan().all()
+    assert torch.equal(got.isnan(), want.isnan()), (int(got.isnan().sum()), int(want.isnan().sum()))
+    over = torch.where(want.isnan(), 0.0, (got - want).abs() - torch.where(bound.isnan(), math.inf, bound))
+    assert bool((over <= 0).all()), float(over.max())
