@@ -343,7 +343,8 @@ int imparo_attention_decode(const void* q, const void* k_cache, const void* v_ca
 // Attention for rows that bring one token each, in groups whose rows have the keys 0 .. shared[g] - 1 in the same pages: those are
 // read once a group, through the table of its first listed row. group_start [n_groups + 1]: group g is the listed rows group_start[g]
 // .. group_start[g + 1] - 1; a listed row in no group shares nothing. Bounds that launches are shaped by, and that must hold: max_shared on
-// shared[g], max_own on the keys a row has behind its group's shared ones, max_group on the rows of a group. The result is the
+// shared[g], max_own on the keys a row has behind its group's shared ones, max_group on the rows of a group (a row past one of them is
+// NaN, unless the launch reaches all of its keys as it is). The result is the
 // softmax over each row's keys 0 .. position (under `window` the last so many of them; a position below 0 sees nothing and gives
 // zeros); weights are rounded to bfloat16 before they meet the values. part_o [n_rows, heads, parts, head_dim] and part_ml [n_rows,
 // heads, parts, 2] float32 hold the results of parts of the keys, with parts = imparo_attention_shared_parts(...); too few of them are IMPARO_SCRATCH_TOO_SMALL.

@@ -68,21 +68,28 @@ struct SharedArgs {
     int n_rows, n_groups, stride, page_shift, heads, kv_heads, per, n_pages, window;      // per: heads a kv head
     int n_pre, pre_split, n_own, own_split;      // parts and keys a part: of the shared keys, of a row's own
     int pre_tiles, own_tiles;                    // blocks' shares of a group's queries of a kv head, and 16 queries of a row's
+    int pre_queries;                             // queries of a kv head that those blocks have room for
     int pre_blocks;                              // blocks for shared keys: the first ones
     float scale;                                 // its size, times log2(e)
     uint32_t flip;                               // its sign, for two bfloat16 of a query at once
 };
 
-// The group a listed row is in (its keys up to `shared` are the group's), or -1. All lanes ask for the same row.
-__device__ __forceinline__ int group_of(const SharedArgs& a, int i) {
+// The group a listed row is in (its keys up to `shared` are the group's), or -1, and its first row. All lanes ask for the same row.
+struct RowGroup {
+    int g, first;
+};
+__device__ __forceinline__ RowGroup group_of(const SharedArgs& a, int i) {
     const int lane = threadIdx.x & (WAVE - 1);
     for (int g0 = 0; g0 < a.n_groups; g0 += WAVE) {
-        const int g = g0 + lane;
-        const bool here = g < a.n_groups && a.group_start[g] <= i && i < a.group_start[g + 1];
+        const int g = g0 + lane, first = g < a.n_groups ? a.group_start[g] : INT32_MAX;
+        const bool here = first <= i && i < a.group_start[min(g, a.n_groups - 1) + 1];
         const unsigned long long who = __ballot(here);
-        if (who) return g0 + __ffsll((long long)who) - 1;
+        if (who) {
+            const int at = __builtin_amdgcn_readfirstlane(__ffsll((long long)who) - 1);
+            return RowGroup{g0 + at, __builtin_amdgcn_readlane(first, at)};
+        }
     }
-    return -1;
+    return RowGroup{-1, 0};
 }
 // 16 bytes of a query, its sign turned where the scale is negative: the largest score is then that of the largest product
 __device__ __forceinline__ u32x4 query_piece(const SharedArgs& a, const bf16_t* q, bool valid) {
@@ -408,7 +415,7 @@ struct OwnWave {
         const int kvh = unit % a.kv_heads, part = unit / a.kv_heads % a.n_own, rest = unit / (a.kv_heads * a.n_own);
         const int first_query = rest % a.own_tiles * 16, i = rest / a.own_tiles;
         if (i >= a.n_rows) return;
-        const int row = a.rows[i], keys = shared_keys(a, group_of(a, i)), t = a.seg_start[row];
+        const int row = a.rows[i], keys = shared_keys(a, group_of(a, i).g), t = a.seg_start[row];
         const int32_t* __restrict__ table = a.table + (size_t)row * a.stride;
         const int begin = (keys & ~(OWN_KEYS - 1)) + part * a.own_split;
         const int pos = min(a.positions[t], keys_of_table(a) - 1);
@@ -557,10 +564,15 @@ __global__ __launch_bounds__(SHARED_WAVES * WAVE) void k_attn_shared_merge(Share
     };
     if (parts) ask(0, parts);
     const int t = a.seg_start[row];
-    const int keys = shared_keys(a, group_of(a, i));
+    const RowGroup group = group_of(a, i);
+    const int keys = shared_keys(a, group.g);
     const int end_all = (int)min((long long)a.positions[t] + 1, (long long)keys_of_table(a));
     const int pre = min((keys + a.pre_split - 1) / a.pre_split, a.n_pre);
     const int own = keys < end_all ? min((end_all - (keys & ~(OWN_KEYS - 1)) + a.own_split - 1) / a.own_split, a.n_own) : 0;
+    // Keys that the launch was not shaped for (a bound of the call's that does not hold for what stands on the device): no block or wave took them, and
+    // what stands in place of their parts is another call's. Such a row is NaN
+    const bool lost = min(keys, end_all) > a.n_pre * a.pre_split || (keys < end_all && end_all - (keys & ~(OWN_KEYS - 1)) > a.n_own * a.own_split) ||
+                      (keys > 0 && (long long)(i + 1 - max(group.first, 0)) * a.per > a.pre_queries);
     auto there = [&](int k) { return k < pre || (k >= a.n_pre && k < a.n_pre + own); };
     // A part in which the row sees nothing is -inf, 0 and zeros; one whose scores are all NaN has no reference either, but a NaN for a sum, and weighs
     // NaN. What a part holds counts even where its weight vanishes beside the others': NaN times 0 is NaN.
@@ -594,7 +606,7 @@ __global__ __launch_bounds__(SHARED_WAVES * WAVE) void k_attn_shared_merge(Share
 #pragma unroll
         for (int j = 0; j < 4; ++j) total[j] += __shfl(acc[j], lane % lanes_a_part + k * lanes_a_part, WAVE);
     if (sub != 0) return;
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;             // a row that sees nothing is zeros
+    const float inv = lost ? __builtin_nanf("") : sum == 0.f ? 0.f : 1.0f / sum;      // (a row that sees nothing is zeros)
     uint2 packed;
     packed.x = f32x2_to_bf16x2(total[0] * inv, total[1] * inv);
     packed.y = f32x2_to_bf16x2(total[2] * inv, total[3] * inv);
@@ -664,7 +676,7 @@ extern "C" int imparo_attention_decode_shared(const void* q, const void* k_cache
     if (blocks > 1 << 30 || own_waves > 1 << 30 || (long long)n_rows * heads > 1 << 30) return IMPARO_BAD_ARGUMENT;
     const SharedArgs a{(const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, (bf16_t*)out, part_o, part_ml, rows, group_start, shared,
                        seg_start, positions, block_table, n_rows, n_groups, table_stride, __builtin_ctz((unsigned)page_size), heads, kv_heads,
-                       heads / kv_heads, n_pages, window, s.n_pre, s.pre_split, s.n_own, s.own_split, s.pre_tiles, s.own_tiles, (int)pre_blocks,
+                       heads / kv_heads, n_pages, window, s.n_pre, s.pre_split, s.n_own, s.own_split, s.pre_tiles, s.own_tiles, s.pre_tiles * 32 * s.query_waves, (int)pre_blocks,
                        fmaxf(fabsf(scale) * 1.44269504088896340736f, 1.0e-37f), scale < 0.f ? 0x80008000u : 0u};
     hipStream_t st = (hipStream_t)stream;
     if (blocks) {

@@ -617,7 +617,7 @@ def attention_decode_shared(q, k_cache, v_cache, out, part_o, part_ml, rows, n_r
     are read once a group, through its first row's table, and the ones behind by each row through its own (so a page in which the shared keys end
     may be a copy in every row); a listed row in no group shares nothing. The bounds shape the launch, so that it can be captured while
     groups, shares and positions change on the device, and must hold: shared[g] <= max_shared, position + 1 - shared[g] <= max_own, rows of
-    a group <= max_group. `part_o` [n_rows, heads, parts, head_dim] and `part_ml` [n_rows, heads, parts, 2] float32 are scratch, parts =
+    a group <= max_group (a row past one of them is NaN, unless the launch reaches all of its keys as it is). `part_o` [n_rows, heads, parts, head_dim] and `part_ml` [n_rows, heads, parts, 2] float32 are scratch, parts =
     attention_shared_parts(...); launches that may run at once, and captured ones that may be replayed at once, need scratch of their own. Softmax
     weights are rounded to bfloat16 before they meet the values. A row whose position is below 0 sees nothing and is zeros; rows that
     are not listed are left as they are."""

@@ -318,3 +318,31 @@ def test_what_is_not_a_number_in_what_a_row_sees(where, scale, heads, kv, dim, p
     assert torch.equal(got.isnan(), want.isnan()), (int(got.isnan().sum()), int(want.isnan().sum()))
     over = torch.where(want.isnan(), 0.0, (got - want).abs() - torch.where(bound.isnan(), math.inf, bound))
     assert bool((over <= 0).all()), float(over.max())
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 2), (48, 1)])
+@pytest.mark.parametrize("broken", [{"max_own": 1}, {"max_own": 0}, {"max_shared": 64}, {"max_shared": 0}, {"max_group": 1}, {"max_group": 0}])
+def test_rows_past_a_bound_are_not_numbers(broken, heads, kv):
+    """Bounds are about numbers on the device, which the host cannot look at. Over scratch that holds what an earlier call might have left there, a
+    row past a bound is NaN as a whole, or right where the launch reached all its keys; the others are right."""
+    dim, page = 64, 32
+    b = Batch([(300, [200, 1, 3] + [2] * 60), (40, [3, 180]), (None, [1, 90])], heads, kv, dim, page, seed=heads)
+    bounds = {**dict(max_shared=b.max_shared, max_own=b.max_own, max_group=b.max_group), **broken}
+    n = b.n + 1
+    parts = ops().attention_shared_parts(b.n, heads, kv, dim, len(b.shared), bounds["max_group"], bounds["max_shared"], bounds["max_own"])
+    out = torch.full((n, heads * dim), 7.0, dtype=torch.bfloat16, device=DEV)
+    part_o, part_ml = torch.full((b.n, heads, parts, dim), 3.0, device=DEV), torch.full((b.n, heads, parts, 2), 5.0, device=DEV)
+    ops().attention_decode_shared(b.q.to(DEV), b.k.to(DEV), b.v.to(DEV), out, part_o, part_ml, ints(b.order), b.n, ints(b.group_start),
+                                  ints(b.shared), ints(np.arange(n)), ints(b.positions + [0]), ints(b.table), b.scale, None, **bounds)
+    got = out[:b.n].cpu().double()
+    want, bound = plain.attend(b.q[:b.n], b.k, b.v, b.tables, b.positions, b.scale)
+    right, lost = ((got - want).abs() <= bound).all(dim=1), got.isnan().all(dim=1)
+    assert bool((right | lost).all()), (~(right | lost)).nonzero().flatten().tolist()
+    in_group = [(g, i - a) for g, (a, e) in enumerate(zip(b.group_start, b.group_start[1:])) for i in range(a, e)]
+    for i in range(b.n):                                       # listed row i
+        g, place = in_group[i] if i < len(in_group) else (None, 0)
+        shared = b.shared[g] if g is not None else 0
+        own = b.positions[b.order[i]] + 1 - shared
+        if shared <= bounds["max_shared"] and own <= bounds["max_own"] and (not shared or place < bounds["max_group"]):
+            assert bool(right[b.order[i]]), i
+    assert bool(lost.any())
