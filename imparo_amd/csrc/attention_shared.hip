@@ -643,7 +643,8 @@ static SharedShape shared_shape(int n_rows, int heads, int kv_heads, int n_group
 }
 static bool shared_sizes_bad(int n_rows, int heads, int kv_heads, int n_groups, int max_group, int max_shared, int max_own) {
     return n_rows < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || n_groups < 0 || max_group < 0 || max_shared < 0 || max_own < 0 ||
-           max_shared > 1 << 30 || max_own > 1 << 30 || n_rows > 65535 || n_groups > 1 << 20 || max_group > 1 << 20 || heads > 1 << 16;
+           max_shared > 1 << 30 || max_own > 1 << 30 || n_rows > 65535 || n_groups > 1 << 20 || max_group > 1 << 20 || heads > 1 << 16 ||
+           (long long)max_group * (heads / kv_heads) > 1 << 30;             // (queries of a kv head are numbered in 32 bits)
 }
 
 extern "C" int imparo_attention_shared_parts(int n_rows, int heads, int kv_heads, int n_groups, int max_group, int max_shared, int max_own) {

@@ -605,6 +605,9 @@ def attention_shared_parts(n_rows: int, heads: int, kv_heads: int, head_dim: int
         raise KernelArgumentError(f"attention_shared_parts: {heads} heads of {head_dim} by {kv_heads} are not taken")
     if min(n_rows, n_groups, max_group, max_shared, max_own) < 0 or max(max_shared, max_own) > 1 << 30:
         raise KernelArgumentError("attention_shared_parts: a bound is negative, or above 2^30")
+    if n_rows > 65535 or n_groups > 1 << 20 or max_group > 1 << 20 or heads > 1 << 16 or max_group * (heads // kv_heads) > 1 << 30:
+        raise KernelArgumentError(f"attention_shared_parts: {n_rows} rows in {n_groups} groups of up to {max_group}, {heads} heads by "
+                                  f"{kv_heads}, are not taken")
     return int(library().imparo_attention_shared_parts(int(n_rows), int(heads), int(kv_heads), int(n_groups), int(max_group),
                                                        int(max_shared), int(max_own)))
 

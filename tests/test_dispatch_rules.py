@@ -48,3 +48,16 @@ def test_attention_under_a_rule_from_the_projections_rows(rows, splits, heads, k
     (1, 16, 8, 128, 1, 0, 1), (1, 8, 8, 64, -20, 0, 1)])
 def test_float32_attention_of_few_tokens(tokens, heads, kv_heads, dim, window, keep, pays):
     assert library().imparo_attention_f32_split_pays(tokens, heads, kv_heads, dim, window, keep) == pays
+
+
+@pytest.mark.parametrize("heads,max_group,taken", [(65536, 1 << 14, True), (65536, (1 << 14) + 1, False), (65536, 1 << 20, False), (1024, 1 << 20, True),
+                                                   (32, (1 << 20) + 1, False), (65537, 1, False)])
+def test_attention_over_a_shared_prefix_numbers_queries_in_32_bits(heads, max_group, taken):
+    from imparo_amd.kernels import KernelArgumentError, ops
+    parts = library().imparo_attention_shared_parts(100, heads, 1, 1, max_group, 100, 100)
+    assert (parts > 0) == taken
+    if taken:
+        assert ops.attention_shared_parts(100, heads, 1, 64, 1, max_group, 100, 100) == parts
+    else:
+        with pytest.raises(KernelArgumentError, match="not taken"):
+            ops.attention_shared_parts(100, heads, 1, 64, 1, max_group, 100, 100)
