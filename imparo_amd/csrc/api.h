@@ -346,7 +346,7 @@ int imparo_attention_decode(const void* q, const void* k_cache, const void* v_ca
 // shared[g], max_own on the keys a row has behind its group's shared ones, max_group on the rows of a group (a row past one of them is
 // NaN, unless the launch reaches all of its keys as it is). The result is the
 // softmax over each row's keys 0 .. position (under `window` the last so many of them; a position below 0 sees nothing and gives
-// zeros); weights are rounded to bfloat16 before they meet the values. part_o [n_rows, heads, parts, head_dim] and part_ml [n_rows,
+// zeros); weights are rounded to bfloat16 before they meet the values and are summed. part_o [n_rows, heads, parts, head_dim] and part_ml [n_rows,
 // heads, parts, 2] float32 hold the results of parts of the keys, with parts = imparo_attention_shared_parts(...); too few of them are IMPARO_SCRATCH_TOO_SMALL.
 int imparo_attention_shared_parts(int n_rows, int heads, int kv_heads, int n_groups, int max_group, int max_shared, int max_own);
 int imparo_attention_decode_shared(const void* q, const void* k_cache, const void* v_cache, void* out, float* part_o,

@@ -52,6 +52,20 @@ __device__ __forceinline__ u32x4 only_between(u32x4 v, int key, int lo, int hi) 
     return v;
 }
 
+// Eight weights added up as they go into the product with the values, two an instruction: the denominator has the same roundings in it. (The
+// instruction rounds a sum of three by up to 1.5e-7 of it, measured.)
+__device__ __forceinline__ float weights_sum(u32x4 p) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 ones = {(__bf16)1.f, (__bf16)1.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t two = p[j];                                // (a cast of the element itself takes the vector's first)
+        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), ones, sum, false);
+    }
+    return sum;
+}
+
 struct SharedArgs {
     const bf16_t* __restrict__ q;
     const bf16_t* __restrict__ k;
@@ -116,7 +130,7 @@ __device__ __forceinline__ bool moved_reference(float& m, float mx, float& corr,
 // ---- shared keys
 // A block's four waves take QW tiles of 32 queries and, for QW of 2, the two halves of a tile of keys. Bound by the exponentials with many queries (16 a lane
 // for 32 keys, a quarter of a lane's rate each, beside 2 ND products), by memory with few. Weights are rounded to bfloat16 for the second product, half a
-// step of 2^-8 each and of either sign; their sum takes them as they were. 32 heads by 8 of 64, 64 rows behind 32,768 keys (256 queries a kv
+// step of 2^-8 each and of either sign, and summed as rounded, so that a key with nearly all the weight gives its value and not that off by half a step. 32 heads by 8 of 64, 64 rows behind 32,768 keys (256 queries a kv
 // head): 44 us with the adding up of parts (47 with the two halves of a tile one after the other), 390 TFLOP/s; 24 by 8 of 128, four groups of
 // 16 rows behind 8,192 keys: 40 us, 3.3 TB/s, a tile's loads a block on their way. Not faster: the sums out of the matrix pipe (one more product a tile where the vector pipe waits as it
 // is), two tiles on their way in registers (they no longer fit), three blocks a CU (more parts to add up).
@@ -295,18 +309,14 @@ struct SharedBlock {
                     const float from = m == -INFINITY ? 0.f : m;
 #pragma unroll
                     for (int n = 0; n < N; ++n) {
-                        float sum = 0.f;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.scale, -from));
-                            sum += s[n][r];
-                        }
-                        l += sum;
+                        for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.scale, -from));
                         SharedFrag p[2];
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
                             p[u].u = u32x4{f32x2_to_bf16x2(s[n][8 * u], s[n][8 * u + 1]), f32x2_to_bf16x2(s[n][8 * u + 2], s[n][8 * u + 3]),
                                            f32x2_to_bf16x2(s[n][8 * u + 4], s[n][8 * u + 5]), f32x2_to_bf16x2(s[n][8 * u + 6], s[n][8 * u + 7])};
+                        l += weights_sum(p[0].u) + weights_sum(p[1].u);
 #pragma unroll
                         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -505,15 +515,11 @@ struct OwnWave {
                     for (int dt = 0; dt < ND; ++dt) o[dt] *= corr;
                 }
                 const float from = m == -INFINITY ? 0.f : m;
-                float sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], a.scale, -from));
-                    sum += s[j];
-                }
-                l += sum;
+                for (int j = 0; j < 8; ++j) s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], a.scale, -from));
                 SharedFrag p;
                 p.u = u32x4{f32x2_to_bf16x2(s[0], s[1]), f32x2_to_bf16x2(s[2], s[3]), f32x2_to_bf16x2(s[4], s[5]), f32x2_to_bf16x2(s[6], s[7])};
+                l += weights_sum(p.u);
 #pragma unroll
                 for (int dt = 0; dt < ND; ++dt) {
                     SharedFrag f;

@@ -622,7 +622,7 @@ def attention_decode_shared(q, k_cache, v_cache, out, part_o, part_ml, rows, n_r
     groups, shares and positions change on the device, and must hold: shared[g] <= max_shared, position + 1 - shared[g] <= max_own, rows of
     a group <= max_group (a row past one of them is NaN, unless the launch reaches all of its keys as it is). `part_o` [n_rows, heads, parts, head_dim] and `part_ml` [n_rows, heads, parts, 2] float32 are scratch, parts =
     attention_shared_parts(...); launches that may run at once, and captured ones that may be replayed at once, need scratch of their own. Softmax
-    weights are rounded to bfloat16 before they meet the values. A row whose position is below 0 sees nothing and is zeros; rows that
+    weights are rounded to bfloat16 before they meet the values and are summed. A row whose position is below 0 sees nothing and is zeros; rows that
     are not listed are left as they are."""
     n, heads, head_dim, n_pages, kv_heads, page_size = _check_mfma(q, k_cache, v_cache, out)
     _here(q, "q")

@@ -346,3 +346,31 @@ def test_rows_past_a_bound_are_not_numbers(broken, heads, kv):
         if shared <= bounds["max_shared"] and own <= bounds["max_own"] and (not shared or place < bounds["max_group"]):
             assert bool(right[b.order[i]]), i
     assert bool(lost.any())
+
+
+def with_values_of_one(b):
+    b.v = torch.where(b.v.isnan(), b.v, torch.ones_like(b.v))
+    return b
+
+
+@pytest.mark.parametrize("heads,kv,dim,page", [(4, 2, 64, 32), (4, 2, 48, 64), (48, 1, 64, 64), (48, 1, 128, 16), (70, 2, 80, 128)])
+@pytest.mark.parametrize("spread", [0.5, 5.0, 30.0])
+def test_values_that_are_all_alike_come_out_as_they_are(spread, heads, kv, dim, page):
+    """A sum of weights over the sum of the same weights, whatever a weight was rounded to: 1 off by no more than float32 sums of some hundred
+    terms are (500 times 1.5e-7, and 500 2^-24), and bfloat16's nearest number to that is 1 (the next one below lies 2^-8 away)."""
+    b = with_values_of_one(Batch([(300, [1, 40, 170]), (0, [33, 260])], heads, kv, dim, page, seed=dim, spread=spread))
+    assert torch.equal(b.run(), torch.ones(b.n, heads * dim, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("heads,kv,dim,page", [(8, 2, 64, 64), (48, 1, 64, 16), (48, 1, 128, 128)])
+@pytest.mark.parametrize("groups,low,high", [([(128, [1] * 8)], 3, 70), ([(None, [64] * 8)], 3, 40)])
+def test_the_same_where_one_key_of_a_later_tile_has_nearly_all_the_weight(groups, low, high, heads, kv, dim, page):
+    """Its weight is then any number up to 2^8 (the reference of the exponentials stays with the first tile's largest score, at `low`), not 1."""
+    b = with_values_of_one(Batch(groups, heads, kv, dim, page, seed=dim))
+    octaves = torch.linspace(4.0, 7.9, (b.n + 1) * heads).view(b.n + 1, heads, 1)          # of the score at `high` above that at `low`
+    b.q = (octaves / (dim * b.scale * math.log2(math.e)) * torch.ones(dim)).to(torch.bfloat16)
+    b.k = torch.where(b.k.isnan(), b.k, -torch.ones_like(b.k))
+    for table in b.tables:
+        b.k[table[low // page], :, low % page] = 0.0
+        b.k[table[high // page], :, high % page] = 1.0
+    assert torch.equal(b.run(), torch.ones(b.n, heads * dim, dtype=torch.bfloat16))
