@@ -374,3 +374,52 @@ def test_the_same_where_one_key_of_a_later_tile_has_nearly_all_the_weight(groups
         b.k[table[low // page], :, low % page] = 0.0
         b.k[table[high // page], :, high % page] = 1.0
     assert torch.equal(b.run(), torch.ones(b.n, heads * dim, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("heads,kv", [(8, 2), (48, 1)])
+def test_a_nan_that_all_rows_see_costs_nothing(heads, kv):
+    """One value of a shared prefix: the products pass it on by themselves. (Sums made anew, key by key, took a hundred times the call's time.)"""
+    b = Batch([(4096, [1, 2, 3, 4])], heads, kv, 64, 64, seed=1)
+    n, dim = b.n + 1, 64
+    bounds = dict(max_shared=b.max_shared, max_own=b.max_own, max_group=b.max_group)
+    parts = ops().attention_shared_parts(b.n, heads, kv, dim, 1, *(bounds[k] for k in ("max_group", "max_shared", "max_own")))
+    out = torch.zeros(n, heads * dim, dtype=torch.bfloat16, device=DEV)
+    part_o, part_ml = torch.empty(b.n, heads, parts, dim, device=DEV), torch.empty(b.n, heads, parts, 2, device=DEV)
+    k, v = b.k.to(DEV), b.v.to(DEV)
+    args = (ints(b.order), b.n, ints(b.group_start), ints(b.shared), ints(np.arange(n)), ints(b.positions + [0]), ints(b.table), b.scale, None)
+    q = b.q.to(DEV)
+
+    def fastest():
+        times = []
+        for _ in range(8):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            for _ in range(10):
+                ops().attention_decode_shared(q, k, v, out, part_o, part_ml, *args, **bounds)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        return min(times)
+
+    clean = fastest()
+    v[b.tables[0][0], :, 3, 5] = float("nan")
+    poisoned = fastest()
+    rows = out[:b.n].view(b.n, heads, dim)
+    assert bool(rows[:, :, 3].isnan().all()) and not rows[:, :, 4:].isnan().any()
+    assert poisoned < 3 * clean, (poisoned, clean)
+
+
+@pytest.mark.parametrize("heads,kv,dim,page", [(8, 2, 64, 32), (48, 1, 64, 64), (48, 1, 128, 16)])
+@pytest.mark.parametrize("spread", [1.5, 5.0, 30.0])
+def test_values_alike_beside_one_that_is_infinite(spread, heads, kv, dim, page):
+    """At a key that two of the rows see: the others' sums are made anew, numerator and denominator out of the same weights."""
+    b = with_values_of_one(Batch([(210, [-150, -60, 4, 30])], heads, kv, dim, page, seed=dim, spread=spread))
+    table = b.tables[int(np.argmax(b.positions))]
+    b.v[table[190 // page], :, 2, 190 % page] = float("inf")
+    want = torch.ones(b.n, heads, dim, dtype=torch.bfloat16)
+    want[torch.tensor(b.positions) >= 190, :, 2] = float("inf")
+    got = b.run().view(b.n, heads, dim)
+    # (a weight below float32's smallest number makes NaN of the infinity)
+    assert torch.equal(torch.where(got[:, :, 2].isnan() & want[:, :, 2].isinf(), want[:, :, 2], got[:, :, 2]), want[:, :, 2])
+    got[:, :, 2] = want[:, :, 2]
+    assert torch.equal(got, want)
