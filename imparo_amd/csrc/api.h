@@ -54,7 +54,7 @@ int imparo_place_tokens(int32_t* ids, const int32_t* dst, const int32_t* src, co
 // wide as the longest need (what lies beyond is left out). seg_start [n_rows]: where a row's tokens begin; positions, row_of_token and (unless
 // null) slots = page * page_size + place in the page (-1 without a page) [n_tokens]: token by token, up to n_tokens of them; what lies behind
 // the last token is left as it is. lists [n_rows]: the rows that bring one token, then those that bring more. counts [4]: tokens, pages taken
-// from `pages` (more than n_pages: there were too few), rows with one token, rows with more. leader and shared both or neither.
+// from `pages` (more than n_pages: there were too few), rows with one token, rows with more. Positions and counts past 2^31 - 1 are that. leader and shared both or neither.
 int imparo_step_tables_max_rows();
 int imparo_step_tables(const int32_t* lengths, const int32_t* new_tokens, const int32_t* leader, const int32_t* shared,
                        const int32_t* pages, int n_pages, int page_size, int n_rows, int32_t* table, int width,

@@ -12,12 +12,14 @@ struct TableRows {
     const int32_t* leader;        // or null: no row takes pages over
     const int32_t* shared;
     int page_shift, n_rows;
-    __device__ __forceinline__ long long length(int r) const { return max(lengths[r], 0); }
+    // (a row's last position and its pages, where they are pages of one token, may pass 2^31: unsigned)
+    __device__ __forceinline__ uint32_t length(int r) const { return (uint32_t)max(lengths[r], 0); }
     __device__ __forceinline__ int brings(int r) const { return max(new_tokens[r], 0); }
-    __device__ __forceinline__ int need(int r) const {
-        return (int)((length(r) + brings(r) + (1 << page_shift) - 1) >> page_shift);
+    __device__ __forceinline__ uint32_t need(int r) const {
+        const uint32_t tokens = length(r) + (uint32_t)brings(r);
+        return (tokens >> page_shift) + ((tokens & ((1u << page_shift) - 1)) != 0);
     }
-    __device__ __forceinline__ int taken(int r) const { return leader ? min(max(shared[r], 0), need(r)) : 0; }
+    __device__ __forceinline__ uint32_t taken(int r) const { return leader ? min((uint32_t)max(shared[r], 0), need(r)) : 0; }
 };
 
 // Every block adds up all rows (a row's first page and first token are sums over the rows before it; a few reads a thread, and no
@@ -83,13 +85,13 @@ __global__ __launch_bounds__(TABLES_THREADS) void k_step_tables(
     __syncthreads();
 
     const int ps = rows.page_shift;
-    auto entry = [&](int row, int j) -> int {                     // what stands at place j of a row's table
+    auto entry = [&](int row, uint32_t j) -> int {                // what stands at place j of a row's table
         if (j >= rows.need(row)) return -1;
         for (int hops = 0; hops < n; ++hops) {
-            const int taken = rows.taken(row);
+            const uint32_t taken = rows.taken(row);
             if (j >= taken) {
                 if (j >= rows.need(row)) return -1;               // (its leader is shorter than what was to be taken over)
-                const long long at = first_page[row] + j - taken;
+                const long long at = first_page[row] + (j - taken);
                 return at < n_pages ? pages[at] : -1;
             }
             row = rows.leader[row];
@@ -99,14 +101,15 @@ __global__ __launch_bounds__(TABLES_THREADS) void k_step_tables(
     };
     const int step = gridDim.y * TABLES_THREADS, at = blockIdx.y * TABLES_THREADS + tid;
     for (int j = at; j < width; j += step) table[(size_t)r * width + j] = entry(r, j);
-    const long long start = start_shared, length = rows.length(r);
+    const long long start = start_shared;
+    const uint32_t length = rows.length(r);
     const int b = rows.brings(r);
     for (int i = at; i < b && start + i < n_tokens; i += step) {
-        const long long pos = length + i;
-        positions[start + i] = (int32_t)pos;
+        const uint32_t pos = length + (uint32_t)i;
+        positions[start + i] = (int32_t)min(pos, (uint32_t)INT32_MAX);
         row_of_token[start + i] = r;
         if (slots) {
-            const int p = entry(r, (int)(pos >> ps));
+            const int p = entry(r, pos >> ps);
             slots[start + i] = p < 0 ? -1 : ((int64_t)p << ps) + (pos & ((1 << ps) - 1));
         }
     }

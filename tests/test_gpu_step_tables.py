@@ -130,3 +130,14 @@ def test_a_step_of_continuations_on_the_device():
         rows = logits.cpu().numpy()
         assert picks.cpu().tolist() == [plain.pick(rows[r], float(temperature[r]), float(u[r]), 0, 0.9) for r in range(n)]
         lengths += 1
+
+
+def test_positions_past_32_bits():
+    """Pages of one token, whose numbers are then positions: a row that grows past 2^31 names the pages there are, and no other row's."""
+    full = lambda *s, dtype=torch.int32: torch.full(s, -7, dtype=dtype, device=DEV)
+    top = 2 ** 31 - 1
+    table, start, positions, row, slots, lists, counts = full(2, 3), full(2), full(4), full(4), full(4, dtype=torch.int64), full(2), full(4)
+    ops().step_tables(ints([top, 4]), ints([3, 1]), ints([8, 6, 4, 2, 0]), 1, table, start, positions, row, slots, lists, counts)
+    assert table.tolist() == [[8, 6, 4], [-1, -1, -1]] and start.tolist() == [0, 3]
+    assert positions.tolist() == [top, top, top, 4] and row.tolist() == [0, 0, 0, 1] and slots.tolist() == [-1] * 4
+    assert lists.tolist() == [1, 0] and counts.tolist() == [4, top, 1, 1]
