@@ -139,7 +139,8 @@ class Sampler:
         if all(t <= 0 for t in temperatures):
             ops.argmax_rows(logits, out)
         else:
-            filtered = filters is not None and any(tuple(f) != NO_FILTERS for f in filters)
+            # (a greedy row's filters are of no bearing on its pick)
+            filtered = filters is not None and any(t > 0 and tuple(f) != NO_FILTERS for t, f in zip(temperatures, filters))
             b.params_host[0, :n] = torch.tensor(list(temperatures), dtype=torch.float32)
             b.params_host[1, :n] = torch.tensor(list(uniforms), dtype=torch.float32)
             if filtered:

@@ -239,3 +239,23 @@ def test_rows_whose_largest_logits_are_all_alike(level, vocab):
     n = len(rows)
     for p, m in ((0.5, 0.0), (0.95, 0.3), (1e-6, 0.0), (1.0 - 2.0 ** -20, 1.0)):
         check(x, [1.0, 0.7] * (n // 2), [0.3, 0.0, 0.9, 0.3, 0.1, 0.7, 0.5, 0.999], [0] * n, [0.9, p] * (n // 2), [0.0, m] * (n // 2))
+
+
+@pytest.mark.parametrize("vocab", [1003, (1 << 19) + 1])
+def test_filters_of_greedy_rows_filter_nothing(vocab, monkeypatch):
+    """Beside rows that are drawn without filters, whose step goes through the kernel without filters and takes rows of any length."""
+    from imparo_amd.sampling.sampler import NO_FILTERS, Sampler
+    from imparo_amd.kernels import ops as o
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((4, vocab)).astype(np.float32)
+    seen, rows = [], o.sample_rows
+    monkeypatch.setattr(o, "sample_rows", lambda *a, **filters: seen.append(filters) or rows(*a, **filters))
+    sampler = Sampler(DEV)
+    t, u = [0.0, 0.9, -1.0, 0.7], [0.5, 0.25, 0.5, 0.75]
+    logits = torch.from_numpy(x).to(DEV)
+    got = sampler.pick(logits, t, u, [(5, 1.0, 0.0), NO_FILTERS, (0, 0.9, 0.1), NO_FILTERS])
+    assert got == sampler.pick(logits, t, u) and seen == [{}, {}]
+    assert got[0] == int(x[0].argmax()) and got[2] == int(x[2].argmax())
+    if vocab < 1 << 19:
+        got = sampler.pick(logits, t, u, [NO_FILTERS, (1, 1.0, 0.0), NO_FILTERS, NO_FILTERS])
+        assert got[1] == int(x[1].argmax()) and list(seen[2]) == ["top_k", "top_p", "min_p"]
