@@ -2,6 +2,7 @@
 // maximum, NaN never wins) and temperature sampling by inverse CDF.
 #include "common.h"
 #include "api.h"
+#include <float.h>
 #include <limits.h>
 
 struct Best {
@@ -1070,7 +1071,7 @@ __global__ __launch_bounds__(PICK_THREADS) void k_pick_rows(
     // what is kept, as a logit: all above `edge`, and so many as it. min-p's own border is the smallest logit that passes it
     float edge = set.key ? float_of(set.key) : -INFINITY;
     int cut = set.cut;
-    float lowest = fmaxf((float)((double)top + floor_y / c1), -3.0e38f);
+    float lowest = fmaxf((float)((double)top + floor_y / c1), -FLT_MAX);      // (-inf where that is out of range, NaN for 0 octaves at an infinite temperature)
     auto next = [](float x, int up) { return float_of(key_of(x) + up); };
     for (int i = 0; i < 8 && weights.octaves(next(lowest, -1)) >= floor_y; ++i) lowest = next(lowest, -1);
     for (int i = 0; i < 16 && weights.octaves(lowest) < floor_y; ++i) lowest = next(lowest, 1);

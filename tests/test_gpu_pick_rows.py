@@ -259,3 +259,18 @@ def test_filters_of_greedy_rows_filter_nothing(vocab, monkeypatch):
     if vocab < 1 << 19:
         got = sampler.pick(logits, t, u, [NO_FILTERS, (1, 1.0, 0.0), NO_FILTERS, NO_FILTERS])
         assert got[1] == int(x[1].argmax()) and list(seen[2]) == ["top_k", "top_p", "min_p"]
+
+
+@pytest.mark.parametrize("vocab", [1003, 16385, 65536])
+@pytest.mark.parametrize("level", [float(np.finfo(np.float32).min), -3.2e38, float(np.finfo(np.float32).max)])
+def test_rows_at_the_ends_of_float32(level, vocab):
+    """A row all of whose logits are a mask's lowest value (or the largest one) picks among them as any row of equal logits does, also
+    where a few are masked by minus infinity; a row with some such masks among ordinary logits leaves them out."""
+    rng = np.random.default_rng(vocab)
+    x = np.full((6, vocab), level, dtype=np.float32)
+    x[1, rng.random(vocab) < 0.3] = -np.inf
+    x[2:4] = np.where(rng.random((2, vocab)) < 0.5, min(level, -level), rng.standard_normal((2, vocab)) * 2).astype(np.float32)
+    x[4, 7] = np.nan
+    u, t = [0.0, 0.6, 0.3, 0.9, 0.999, 1.0], [1.0, 0.7, 1.0, 0.5, 1e3, 1.0]
+    for k, p, m in ((0, 0.9, 0.0), (0, 0.5, 0.3), (0, 1.0, 0.5), (400, 1.0, 0.0), (700, 0.9, 0.0), (400, 0.5, 1.0)):
+        check(x, t, u, [k] * 6, [p] * 6, [m] * 6)
