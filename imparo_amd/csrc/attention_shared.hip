@@ -683,7 +683,7 @@ extern "C" int imparo_attention_decode_shared(const void* q, const void* k_cache
     if (!q || !k_cache || !v_cache || !out || !rows || !seg_start || !positions || !block_table ||
         shared_sizes_bad(n_rows, heads, kv_heads, n_groups, max_group, max_shared, max_own) || (n_groups && (!group_start || !shared)) ||
         table_stride <= 0 || page_size < 16 || page_size > 1 << 20 || (page_size & (page_size - 1)) || head_dim <= 0 || head_dim > 128 || head_dim % 16 ||
-        n_pages <= 0 || window < 0)
+        n_pages <= 0 || window < 0 || !(fabsf(scale) * 1.44269504088896340736f < INFINITY))
         return IMPARO_BAD_ARGUMENT;
     if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)part_o) & 15 || ((uintptr_t)part_ml | (uintptr_t)out) & 7)
         return IMPARO_BAD_ARGUMENT;

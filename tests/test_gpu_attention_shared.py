@@ -423,3 +423,10 @@ def test_values_alike_beside_one_that_is_infinite(spread, heads, kv, dim, page):
     assert torch.equal(torch.where(got[:, :, 2].isnan() & want[:, :, 2].isinf(), want[:, :, 2], got[:, :, 2]), want[:, :, 2])
     got[:, :, 2] = want[:, :, 2]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3.4e38])
+def test_scales_that_are_no_numbers_are_refused(scale):
+    """(The smallest scale stands for 0, and would for a NaN.)"""
+    with pytest.raises(ops().KernelArgumentError):
+        Batch([(32, [4, 4])], 4, 2, 64, 32, seed=1).run(scale=scale)
