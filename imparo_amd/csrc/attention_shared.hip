@@ -131,10 +131,11 @@ __device__ __forceinline__ bool moved_reference(float& m, float mx, float& corr,
 // ---- shared keys
 // A block's four waves take QW tiles of 32 queries and, for QW of 2, the two halves of a tile of keys. Bound by the exponentials with many queries (16 a lane
 // for 32 keys, a quarter of a lane's rate each, beside 2 ND products), by memory with few. Weights are rounded to bfloat16 for the second product, half a
-// step of 2^-8 each and of either sign, and summed as rounded, so that a key with nearly all the weight gives its value and not that off by half a step. 32 heads by 8 of 64, 64 rows behind 32,768 keys (256 queries a kv
-// head): 44 us with the adding up of parts (47 with the two halves of a tile one after the other), 390 TFLOP/s; 24 by 8 of 128, four groups of
-// 16 rows behind 8,192 keys: 40 us, 3.3 TB/s, a tile's loads a block on their way. Not faster: the sums out of the matrix pipe (one more product a tile where the vector pipe waits as it
-// is), two tiles on their way in registers (they no longer fit), three blocks a CU (more parts to add up).
+// step of 2^-8 each and of either sign, and summed as rounded, so that a key with nearly all the weight gives its value and not that off by half a step.
+// 32 heads by 8 of 64, 64 rows behind 32,768 keys (256 queries a kv head): 45 to 47 us with the adding up of parts (3 more with the two halves of a tile
+// one after the other), 380 TFLOP/s; 24 by 8 of 128, four groups of 16 rows behind 8,192 keys: 39 us without it, 3.3 TB/s, a tile's loads a block on
+// their way. Not faster: the sums out of the matrix pipe (one more product a tile where the vector pipe waits as it is), two tiles on their way in
+// registers (they did not fit), three blocks a CU (more parts to add up).
 template <int ND, int QW, bool PAGED>
 struct SharedBlock {
     static constexpr int D = ND * 16, DT = (ND + 1) / 2, THREADS = SHARED_WAVES * WAVE, KW = SHARED_WAVES / QW;
@@ -553,7 +554,7 @@ struct OwnWave {
 };
 
 template <int ND, int QW, bool PAGED>
-__global__ __launch_bounds__(SHARED_WAVES * WAVE, ND > 6 ? 2 : ND > 4 ? 2 : ND > 2 ? 3 : 4) void k_attn_shared(SharedArgs a) {
+__global__ __launch_bounds__(SHARED_WAVES * WAVE, ND > 4 ? 2 : ND > 2 ? 3 : 4) void k_attn_shared(SharedArgs a) {
     typedef SharedBlock<ND, QW, PAGED> Block;
     typedef OwnWave<ND, PAGED> Own;
     __shared__ __attribute__((aligned(16))) char lds[Block::LDS > SHARED_WAVES * Own::LDS ? Block::LDS : SHARED_WAVES * Own::LDS];

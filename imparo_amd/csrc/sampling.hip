@@ -280,10 +280,11 @@ extern "C" int imparo_sample_rows(const float* logits, const float* temperature,
 // token compared with every other where they are few, else by histograms over nine bits of keys or indices at a time (list_find). A row
 // that keeps more than a few under top-p lists the tokens of the border's bin only, has the sums of the ones above by the runs they are in (every wave has a
 // histogram of its run), and picks in the run that u falls in: one exponential a logit, and one for those of that run. What fits neither (large top-k, thousands of ties) is done over the row itself, pass by pass (pick_narrow).
-// Measured, a row a block: one of 65,536 under top-k (and top-p) 12.3 us, under min-p 10.4, under top-p 24 where hardly any are kept, 28 with hundreds,
-// 34 to 39 with thousands (of which the largest 6, weights and their histogram 13, the border's tokens 5 to 9, border and pick 4 to 11); 64 rows
-// under top-k and top-p 15; 256 rows of 130,001 of all kinds 82, under top-k 46.
-#define PICK_THREADS 1024          // of short rows too: 5 of 1,003 under top-k with 256 threads 13.1 us, so 9.9; 8 of 16,000 under top-p 53 and 24
+// Measured, a row a block, logits of normal noise: one of 65,536 under top-k (and top-p) 12.0 us, under min-p 9.4 to 10, under top-p (0.95, T = 1) 23 where
+// one token is kept (a deviation of 6), 25 with 42 (4), 33 with 3,570 (3), 36 to 39 with more (2.5 and less), of which the largest logit 6, weights and
+// their histogram 13, the border's tokens 5 to 9, border and pick 4 to 11; 64 rows under top-k and top-p 13 to 14; 256 rows of 130,001 of all kinds 82, under
+// top-k 43, where argmax takes 52.
+#define PICK_THREADS 1024          // of short rows too (with 256 threads, when that was tried: 5 of 1,003 under top-k 13.1 us for 9.9, 8 of 16,000 under top-p 53 for 24)
 #define PICK_BINS 2048
 #define PICK_BITS 9                // bits of a key or an index that a search in the list settles at a time
 #define PICK_FEW 256               // tokens that are compared with one another instead

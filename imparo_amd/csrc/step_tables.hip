@@ -25,8 +25,8 @@ struct TableRows {
 // Every block adds up all rows (a row's first page and first token are sums over the rows before it; a few reads a thread, and no
 // second launch), then fills one row's table and tokens, a share of them where rows are long (grid y). An entry that a row
 // takes over is looked up in its leader's own pages, through the leader's leader where that one took it over too. Bound by its launch and the
-// trips to memory behind one another (lengths, sums through LDS, pages): 8 rows 5.1 us, 64 rows of 2,080 pages with portions of up to 512 tokens
-// 8.4, 256 rows of 4,097 pages (4 MB of tables) 9.5.
+// trips to memory behind one another (lengths, sums through LDS, pages): 8 rows 4.8 us, 64 rows of 2,080 pages with portions of up to 512 tokens
+// 8.2, 256 rows of 4,097 pages (4 MB of tables) 9.0.
 __global__ __launch_bounds__(TABLES_THREADS) void k_step_tables(
     TableRows rows, const int32_t* __restrict__ pages, int n_pages, int32_t* __restrict__ table, int width,
     int32_t* __restrict__ seg_start, int32_t* __restrict__ positions, int32_t* __restrict__ row_of_token,
